@@ -7,6 +7,7 @@ or a non-sm_100 device raises instead of silently computing elsewhere.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -89,6 +90,19 @@ SIGNATURES = {
     "fp_pattention_routed_fwd": (_c_int, [_c_p, _c_i64, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
                                           _c_int, _c_int, _c_p, _c_p, _c_p, _c_int, _c_int, _c_p, _c_int, _c_p,
                                           _c_sz, _c_p]),
+    "fp_mxfp8_quantize": (_c_int, [_c_p, _c_int, _c_i64, _c_p, _c_p, _c_p]),
+    "fp_mxfp8_dequantize": (_c_int, [_c_p, _c_p, _c_int, _c_i64, _c_p, _c_p]),
+    "fp_swiglu_fwd_mxfp8": (_c_int, [_c_p, _c_p, _c_int, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "fp_swiglu_bwd_mxfp8": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_i64, _c_p, _c_p, _c_p, _c_p]),
+    "fp_router_scores_train": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_i64, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p,
+                                        _c_p, _c_p]),
+    "fp_router_scores_bwd_workspace_size": (_c_sz, [_c_i64, _c_int, _c_int]),
+    "fp_router_scores_bwd": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_i64, _c_int, _c_int,
+                                      _c_p, _c_p, _c_p, _c_int, _c_p, _c_sz, _c_p]),
+    "fp_balance_workspace_size": (_c_sz, [_c_i64, _c_int]),
+    "fp_balance_loss_fwd": (_c_int, [_c_p, _c_i64, _c_int, _c_int, _c_f, _c_p, _c_p, _c_p, _c_int, _c_p, _c_p, _c_p,
+                                     _c_p, _c_p, _c_sz, _c_p]),
+    "fp_balance_loss_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_int, _c_f, _c_p, _c_p, _c_p, _c_p, _c_p]),
 }
 
 _lock = threading.Lock()
@@ -155,6 +169,11 @@ def require_cuda(*tensors: Optional[torch.Tensor]) -> torch.device:
     if dev is None:
         raise RuntimeError("no CUDA tensor given")
     return dev
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current device (launches go to the current device's streams)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def contig(t: torch.Tensor) -> torch.Tensor:

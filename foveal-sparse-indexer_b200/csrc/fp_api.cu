@@ -108,6 +108,8 @@ T* at(void* ws, size_t off) { return reinterpret_cast<T*>(reinterpret_cast<char*
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+}  // namespace
+
 // Every launching entry point starts here.  Launch checks read the runtime's per-thread last error, so a
 // non-sticky error left by earlier, unrelated calls of the caller's thread is cleared first (a sticky
 // error, such as a fault of the context, still fails every launch).
@@ -132,6 +134,8 @@ int device_info(int& num_sms) {
   num_sms = sms;
   return major == 10 ? FP_OK : FP_ERR_DEVICE;
 }
+
+namespace {
 
 // SM count the split-K choice of the workspace layout is made for; kMaxSms when no device can be queried
 // (a layout for more splits is never smaller).

@@ -45,12 +45,16 @@ constexpr int kGemmThreads = 192; // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
 constexpr int kGuN = 256;
 constexpr int kGuStages = 4;
 
+// ---- api.cu
+// SM count of the current device; clears a stale non-sticky error.  FP_ERR_DEVICE when it is no sm_100 GPU.
+int device_info(int& num_sms);
+
 // ---- router.cu
 // k16f_cos (optional): fp32 block keys [NB, 16] of the cosine form (both sides L2-normalised,
-// compute_block_scores core.py:254-266) used instead of k16.
+// compute_block_scores core.py:254-266) used instead of k16.  rnorm (optional): [M] factors 1 / rms(x Wq^T).
 int launch_router_scores(const void* x, const void* wq, const void* k16, int dtype, int64_t M, int D,
                          int NB, float temperature, float* scores, float* q16, cudaStream_t st,
-                         const float* k16f_cos = nullptr);
+                         const float* k16f_cos = nullptr, float* rnorm = nullptr);
 struct SelectOut;
 int launch_select(const float* scores, int64_t M, int NB, int base, float top_p, int k_min, int k_max,
                   int capacity, float temperature, int32_t* idx, int32_t* cnt, const float* k16f,

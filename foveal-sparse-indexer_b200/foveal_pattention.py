@@ -29,6 +29,8 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import kernels
+from ._lib import on_device
+from .training import balance_loss, check_checkpoint, router_scores
 
 
 def _chunk_plan(M: int, ch: int) -> list:
@@ -61,19 +63,29 @@ class _PooledTrain(torch.autograd.Function):
     plus the additive stream out_proj(softmax(S/T) K_16).  Backward: the fused SwiGLU backward kernel
     (``fp_swiglu_bwd``, replacing the reference's Triton ``_swiglu_bwd_kernel``, pattention_triton.py:49-96)
     between plain GEMMs over the gathered active rows, and the chain rule of the additive stream through
-    the softmax, the 16-D scores and the RMSNorm of the query into q_proj, block_keys, out_proj and x."""
+    the softmax, the 16-D scores and the RMSNorm of the query into q_proj, block_keys, out_proj and x.
+
+    With ``module.checkpoint == "mxfp8"`` an 8-bit copy of x is saved instead of x (1.03 bytes an element) and
+    every product of the backward pass that reads x reads the copy's values; the router's part of it is the
+    scores' gradient kernel (``fp_router_scores_bwd``)."""
 
     @staticmethod
     def forward(ctx, module, x2d, k_gate, k_up, v, wq, k16, wout):
         packed = module._packed()
-        scores, _ = kernels.router_scores(x2d, wq, k16)
+        keep = module.checkpoint is not None
+        if keep:
+            scores, q16, rnorm, buf = kernels.router_scores_train(x2d, wq, k16, keep_mxfp8=True)
+        else:
+            scores, _ = kernels.router_scores(x2d, wq, k16)
         active, _ = kernels.pooled_route(None, wq, k16, base_blocks=module.base_blocks,
                                          remote_blocks=module.remote_blocks, mode=1, token_scores=scores,
                                          dtype=x2d.dtype, D=x2d.shape[1])
         _, _, c16, _ = kernels.select(scores, base_blocks=module.base_blocks, top_p=1.0, min_remote=0, max_remote=0,
                                       capacity=0, temperature=module.temperature, block_keys=k16, want_routes=False)
         y = kernels.pooled_forward(x2d, k_gate, k_up, v, packed, active, ctx16=c16, out_proj=wout)
-        ctx.save_for_backward(x2d, k_gate, k_up, v, wq, k16, wout, scores, active)
+        ctx.x_shape, ctx.x_dtype = x2d.shape, x2d.dtype
+        ctx.save_for_backward(buf if keep else x2d, k_gate, k_up, v, wq, k16, wout, scores, active,
+                              *((q16, rnorm) if keep else ()))
         ctx.temperature = module.temperature
         ctx.block_size = module.block_size
         ctx.mark_non_differentiable(scores, active)
@@ -81,8 +93,11 @@ class _PooledTrain(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, _dscores, _dactive):
-        x, kg, ku, v, wq, k16, wout, S, active = ctx.saved_tensors
+        x, kg, ku, v, wq, k16, wout, S, active, *router = ctx.saved_tensors
         T, bs = ctx.temperature, ctx.block_size
+        buf = None
+        if router:
+            buf, x = x, kernels.mxfp8_dequantize(x, ctx.x_shape, ctx.x_dtype)
         M, D = x.shape
         dt = x.dtype
         dy = dy.reshape(M, D).to(dt).contiguous()
@@ -96,14 +111,19 @@ class _PooledTrain(torch.autograd.Function):
         dku = torch.zeros_like(ku).index_copy_(0, idx, (dU.t() @ x).to(ku.dtype))
         dv = torch.zeros_like(v).index_copy_(0, idx, (H.t() @ dy).to(v.dtype))
         # additive stream and router (fp32, as the forward's router): S = rms_norm(x Wq^T) K16^T / 4
-        xf, dyf = x.float(), dy.float()
-        k16f, wqf, woutf = k16.detach().float(), wq.detach().float(), wout.detach().float()
+        dyf = dy.float()
+        k16f, woutf = k16.detach().float(), wout.detach().float()
         soft = torch.softmax(S / T, dim=-1)
         dwout = dyf.t() @ (soft @ k16f)
         dctx = dyf @ woutf
         dk16 = soft.t() @ dctx
         dsoft = dctx @ k16f.t()
         dS = soft * (dsoft - (dsoft * soft).sum(dim=-1, keepdim=True)) / T
+        if router:
+            dx_r, dwq, dk16_r = kernels.router_scores_bwd(dS, None, buf, wq.detach(), k16.detach(), *router, dt)
+            return (None, dx.add_(dx_r).to(dt), dkg, dku, dv, dwq.to(wq.dtype), (dk16 + dk16_r).to(k16.dtype),
+                    dwout.to(wout.dtype))
+        xf, wqf = x.float(), wq.detach().float()
         q = xf @ wqf.t()
         r = torch.rsqrt((q * q).mean(dim=-1, keepdim=True) + torch.finfo(torch.float32).eps)
         qn = q * r
@@ -147,6 +167,7 @@ class FovealPattentionMLP(nn.Module):
         top_p: float = 0.9,
         min_remote_blocks: int = 0,
         max_remote_blocks: Optional[int] = None,
+        checkpoint: Optional[str] = None,
         device=None,
     ):
         super().__init__()
@@ -174,6 +195,8 @@ class FovealPattentionMLP(nn.Module):
         self.top_p = top_p
         self.min_remote_blocks = min_remote_blocks
         self.max_remote_blocks = remote_blocks if max_remote_blocks is None else max_remote_blocks
+        # "mxfp8": training keeps 8-bit copies of the layer input between forward and backward
+        self.checkpoint = check_checkpoint(checkpoint)
 
         fk = dict(dtype=dtype, device=device)
         self.k_gate = nn.Parameter(torch.empty(intermediate_dim, hidden_dim, **fk))
@@ -300,6 +323,25 @@ class FovealPattentionMLP(nn.Module):
         x2d = x.reshape(-1, shape[-1]).to(self.k_gate.dtype)
         s, _ = kernels.router_scores(x2d, self.q_proj_16d.weight.detach(), self.block_keys_16d.detach())
         return s.reshape(*shape[:-1], self.num_blocks)
+
+    def balance_loss(self, x: Tensor, valid: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        """Load-balance loss of the token routes of ``x`` [..., D] and the blocks' slot counts (int64 [NB]).
+
+        The routes are the ones ``routing="token"`` takes (``top_p``, ``min_remote_blocks``,
+        ``max_remote_blocks``); the loss reaches x, q_proj_16d and block_keys_16d through the router scores.
+        ``valid`` (bool [...]) leaves out padding.  Add a small multiple to the training loss to keep the
+        blocks' loads even; see :func:`training.balance_loss`."""
+        xx = x.to(self.k_gate.dtype)
+        scores = router_scores(xx, self.q_proj_16d.weight, self.block_keys_16d, checkpoint=self.checkpoint)
+        s2d = scores.detach().reshape(-1, self.num_blocks)
+        cap = max(int(self.max_remote_blocks), 1)
+        with on_device(s2d.device):
+            idx, cnt, _, _ = kernels.select(s2d, base_blocks=self.base_blocks, top_p=self.top_p,
+                                            min_remote=self.min_remote_blocks, max_remote=self.max_remote_blocks,
+                                            capacity=cap, temperature=self.temperature)
+        lead = x.shape[:-1]
+        return balance_loss(scores, idx.view(*lead, cap), cnt.view(lead), base_blocks=self.base_blocks,
+                            temperature=self.temperature, valid=valid)
 
     # ------------------------------------------------------------------ helpers
     def _packed(self):

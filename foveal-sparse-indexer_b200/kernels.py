@@ -143,6 +143,180 @@ def swiglu_fwd(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
     return h
 
 
+# ---------------------------------------------------------------------------------------------------
+# Training operators: MXFP8 activation copies, router score gradient, load balance
+# ---------------------------------------------------------------------------------------------------
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned (a copy when it is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def mxfp8_nbytes(n: int) -> int:
+    """Bytes of an n-element MXFP8 copy: codes, padded to 16 bytes, then one scale byte per 32 elements."""
+    return (n + 15) // 16 * 16 + (n + 31) // 32
+
+
+def _mx_ptrs(buf: torch.Tensor, n: int, at: int = 0):
+    p = buf.data_ptr() + at
+    return ctypes.c_void_p(p), ctypes.c_void_p(p + (n + 15) // 16 * 16)
+
+
+def mxfp8_quantize(x: torch.Tensor) -> torch.Tensor:
+    """MXFP8 copy of ``x`` (``fp_mxfp8_quantize``): a uint8 buffer of :func:`mxfp8_nbytes` bytes."""
+    dev = require_cuda(x)
+    dt = dtype_code(x.dtype)
+    x = _dense(x)
+    n = x.numel()
+    with _lib.on_device(dev):
+        buf = torch.empty(mxfp8_nbytes(n), dtype=torch.uint8, device=dev)
+        check(_lib.load().fp_mxfp8_quantize(ptr(x), dt, n, *_mx_ptrs(buf, n), stream_handle(dev)), "fp_mxfp8_quantize")
+    return buf
+
+
+def mxfp8_dequantize(buf: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
+    """The values of an MXFP8 copy (``fp_mxfp8_dequantize``) in ``dtype`` and ``shape``."""
+    dev = require_cuda(buf)
+    dt = dtype_code(dtype)
+    with _lib.on_device(dev):
+        y = torch.empty(shape, dtype=dtype, device=dev)
+        n = y.numel()
+        if buf.dtype != torch.uint8 or buf.numel() != mxfp8_nbytes(n):
+            raise ValueError(f"an MXFP8 copy of {n} elements is {mxfp8_nbytes(n)} uint8, got {buf.numel()} {buf.dtype}")
+        check(_lib.load().fp_mxfp8_dequantize(*_mx_ptrs(_dense(buf), n), dt, n, ptr(y), stream_handle(dev)),
+              "fp_mxfp8_dequantize")
+    return y
+
+
+def swiglu_fwd_mxfp8(g: torch.Tensor, u: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """h = silu(g) * u and the MXFP8 copies of g, then u, in one uint8 buffer (``fp_swiglu_fwd_mxfp8``)."""
+    dev = require_cuda(g, u)
+    if g.shape != u.shape:
+        raise ValueError(f"g and u must have the same shape, got {tuple(g.shape)} and {tuple(u.shape)}")
+    dt = dtype_code(g.dtype)
+    g, u = _dense(g), _dense(u.to(g.dtype))
+    n = g.numel()
+    half = (mxfp8_nbytes(n) + 15) // 16 * 16
+    with _lib.on_device(dev):
+        h = torch.empty_like(g)
+        buf = torch.empty(2 * half, dtype=torch.uint8, device=dev)
+        check(_lib.load().fp_swiglu_fwd_mxfp8(ptr(g), ptr(u), dt, n, ptr(h), *_mx_ptrs(buf, n), *_mx_ptrs(buf, n, half),
+                                              stream_handle(dev)), "fp_swiglu_fwd_mxfp8")
+    return h, buf
+
+
+def swiglu_bwd_mxfp8(dout: torch.Tensor, buf: torch.Tensor, want_h: bool = False):
+    """Backward of :func:`swiglu_fwd_mxfp8` (``fp_swiglu_bwd_mxfp8``): (dg, du, h or None), dout's dtype."""
+    dev = require_cuda(dout, buf)
+    dt = dtype_code(dout.dtype)
+    dout = _dense(dout)
+    n = dout.numel()
+    half = (mxfp8_nbytes(n) + 15) // 16 * 16
+    if buf.dtype != torch.uint8 or buf.numel() != 2 * half:
+        raise ValueError("the buffer is not that of swiglu_fwd_mxfp8 for as many elements")
+    with _lib.on_device(dev):
+        dg, du = torch.empty_like(dout), torch.empty_like(dout)
+        h = torch.empty_like(dout) if want_h else None
+        check(_lib.load().fp_swiglu_bwd_mxfp8(ptr(dout), *_mx_ptrs(buf, n), *_mx_ptrs(buf, n, half), dt, n, ptr(dg),
+                                              ptr(du), ptr(h), stream_handle(dev)), "fp_swiglu_bwd_mxfp8")
+    return dg, du, h
+
+
+def router_scores_train(x2d: torch.Tensor, q_proj: torch.Tensor, block_keys: torch.Tensor, keep_mxfp8: bool = False):
+    """:func:`router_scores` for training (``fp_router_scores_train``): (scores [M, NB], q16 [M, 16],
+    rnorm [M], MXFP8 copy of x or None)."""
+    dev = require_cuda(x2d, q_proj, block_keys)
+    dt = dtype_code(x2d.dtype)
+    x2d, q_proj, block_keys = _dense(x2d), _dense(q_proj.to(x2d.dtype)), _dense(block_keys.to(x2d.dtype))
+    M, D = x2d.shape
+    NB = block_keys.shape[0]
+    with _lib.on_device(dev):
+        scores = torch.empty(M, NB, dtype=torch.float32, device=dev)
+        saved = torch.empty(17 * M, dtype=torch.float32, device=dev)
+        q16, rnorm = saved[:16 * M].view(M, 16), saved[16 * M:]
+        buf = torch.empty(mxfp8_nbytes(M * D), dtype=torch.uint8, device=dev) if keep_mxfp8 else None
+        codes, scales = _mx_ptrs(buf, M * D) if keep_mxfp8 and M > 0 else (None, None)
+        check(_lib.load().fp_router_scores_train(ptr(x2d), ptr(q_proj), ptr(block_keys), dt, M, D, NB, ptr(scores),
+                                                 ptr(q16), ptr(rnorm), codes, scales, stream_handle(dev)),
+              "fp_router_scores_train")
+    return scores, q16, rnorm, buf
+
+
+def router_scores_bwd(dscores: torch.Tensor, x2d: Optional[torch.Tensor], buf: Optional[torch.Tensor],
+                      q_proj: torch.Tensor, block_keys: torch.Tensor, q16: torch.Tensor, rnorm: torch.Tensor,
+                      dtype: torch.dtype, grad_dtype: torch.dtype = torch.float32,
+                      want: Tuple[bool, bool, bool] = (True, True, True)):
+    """Gradient of the router scores (``fp_router_scores_bwd``): (dx, dq_proj, dblock_keys), None where not
+    ``want``ed.  The tokens come from ``x2d`` or, where given, from their MXFP8 copy ``buf``; ``dtype`` is
+    theirs."""
+    dev = require_cuda(dscores, x2d, buf, q_proj, block_keys, q16, rnorm)
+    dt = dtype_code(dtype)
+    dscores = _dense(dscores.float())
+    q_proj, block_keys = _dense(q_proj.to(dtype)), _dense(block_keys.to(dtype))
+    x2d = _dense(x2d) if x2d is not None else None
+    q16, rnorm = _dense(q16), _dense(rnorm)
+    (M, NB), D = dscores.shape, q_proj.shape[1]
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        dx = torch.empty(M, D, dtype=dtype, device=dev) if want[0] else None
+        dw = torch.empty(16, D, dtype=grad_dtype, device=dev) if want[1] else None
+        dk = torch.empty(NB, 16, dtype=grad_dtype, device=dev) if want[2] else None
+        if M == 0:
+            return dx, dw.zero_() if dw is not None else None, dk.zero_() if dk is not None else None
+        nbytes = lib.fp_router_scores_bwd_workspace_size(M, D, NB)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        codes, scales = _mx_ptrs(buf, M * D) if buf is not None else (None, None)
+        check(lib.fp_router_scores_bwd(ptr(dscores), ptr(x2d), codes, scales, ptr(q_proj), ptr(block_keys), ptr(q16),
+                                       ptr(rnorm), dt, M, D, NB, ptr(dx), ptr(dw), ptr(dk), dtype_code(grad_dtype),
+                                       ptr(ws), nbytes, stream_handle(dev)), "fp_router_scores_bwd")
+    return dx, dw, dk
+
+
+def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[torch.Tensor],
+                     remote_counts: Optional[torch.Tensor], num_blocks: int, base_blocks: int, temperature: float,
+                     valid: Optional[torch.Tensor], counts_in: Optional[torch.Tensor] = None):
+    """Counts of the routed blocks and, where ``scores`` [M, NB] fp32 are given, the balance loss
+    (``fp_balance_loss_fwd``): (loss 0-d fp32 or None, counts [NB] int64, state [NB + 1] fp32 or None)."""
+    dev = require_cuda(scores, remote_indices, remote_counts, valid, counts_in)
+    scores = _dense(scores) if scores is not None else None
+    idx = _dense(remote_indices.to(torch.int32)) if remote_indices is not None else None
+    cnt = _dense(remote_counts.to(torch.int32)) if remote_counts is not None else None
+    valid = _dense(valid) if valid is not None else None
+    counts_in = _dense(counts_in.to(torch.int64)) if counts_in is not None else None
+    M = scores.shape[0] if scores is not None else cnt.shape[0]
+    cap = idx.shape[1] if idx is not None else 0
+    if cap == 0:  # no list to read; an empty tensor has no address
+        idx = cnt
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        counts = torch.empty(num_blocks, dtype=torch.int64, device=dev)
+        out = torch.empty(num_blocks + 2, dtype=torch.float32, device=dev) if scores is not None else None
+        loss, state = (out[0], out[1:]) if out is not None else (None, None)
+        nbytes = lib.fp_balance_workspace_size(M, num_blocks)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        check(lib.fp_balance_loss_fwd(ptr(scores), M, num_blocks, int(base_blocks), float(temperature), ptr(valid),
+                                      ptr(idx), ptr(cnt), cap, ptr(counts_in), ptr(counts), ptr(loss), ptr(state),
+                                      ptr(ws), nbytes, stream_handle(dev)), "fp_balance_loss_fwd")
+    return loss, counts, state
+
+
+def balance_loss_bwd(scores: torch.Tensor, base_blocks: int, temperature: float, valid: Optional[torch.Tensor],
+                     state: torch.Tensor, dloss: torch.Tensor) -> torch.Tensor:
+    """dscores [M, NB] of :func:`balance_loss_fwd` (``fp_balance_loss_bwd``)."""
+    dev = require_cuda(scores, valid, state, dloss)
+    scores = _dense(scores)
+    valid = _dense(valid) if valid is not None else None
+    dloss = dloss.float()
+    M, NB = scores.shape
+    with _lib.on_device(dev):
+        ds = torch.empty_like(scores)
+        check(_lib.load().fp_balance_loss_bwd(ptr(scores), M, NB, int(base_blocks), float(temperature), ptr(valid),
+                                              ptr(state), ptr(dloss), ptr(ds), stream_handle(dev)),
+              "fp_balance_loss_bwd")
+    return ds
+
+
 PATTENTION_ACTIVATIONS = {"swiglu": 0, "silu": 1, "gelu": 2, "relu": 3, "relu2": 4}
 
 

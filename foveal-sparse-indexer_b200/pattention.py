@@ -28,9 +28,11 @@ from typing import Optional
 
 import torch
 from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
 
 from . import kernels
 from ._lib import require_cuda
+from .training import check_checkpoint
 
 ACTIVATIONS = tuple(kernels.PATTENTION_ACTIVATIONS)
 
@@ -50,9 +52,32 @@ class TritonFusedSwiGLUFunction(torch.autograd.Function):
         return dg, du
 
 
-def triton_fused_swiglu(g: Tensor, u: Tensor) -> Tensor:
-    """SwiGLU of two pre-activation tensors (pattention_triton.py:98-104), differentiable."""
+class _SwiGLUCheckpoint(torch.autograd.Function):
+    """h = silu(g) * u whose backward reads 8-bit copies of g and u."""
+
+    @staticmethod
+    def forward(ctx, g, u):
+        h, buf = kernels.swiglu_fwd_mxfp8(g, u)
+        ctx.u_dtype = u.dtype
+        ctx.save_for_backward(buf)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        buf, = ctx.saved_tensors
+        dg, du, _ = kernels.swiglu_bwd_mxfp8(dh, buf)
+        return dg, du.to(ctx.u_dtype)
+
+
+def triton_fused_swiglu(g: Tensor, u: Tensor, *, checkpoint: Optional[str] = None) -> Tensor:
+    """SwiGLU of two pre-activation tensors (pattention_triton.py:98-104), differentiable.  With
+    ``checkpoint="mxfp8"`` the backward pass reads 8-bit copies of g and u (same h; half of bf16's bytes
+    are held between the passes) and the gradients are those at the copies' values."""
+    check_checkpoint(checkpoint)
     require_cuda(g, u)
+    if checkpoint is not None and torch.is_grad_enabled() and (g.requires_grad or u.requires_grad):
+        return _SwiGLUCheckpoint.apply(g, u)
     return TritonFusedSwiGLUFunction.apply(g, u)
 
 

@@ -1,0 +1,205 @@
+"""Training operators of the routed parameter-block layers.
+
+* ``checkpoint_mxfp8(x)`` keeps an activation in 8 bits from a forward to its backward pass; ``restore()``
+  reads it back.  ``checkpoint="mxfp8"`` of ``triton_fused_swiglu``, ``router_scores`` and
+  ``FovealPattentionMLP`` makes their backward passes read such copies instead of the tensors themselves.
+* ``router_scores(x, q_proj, block_keys)`` is ``compute_router_scores`` (foveal_pattention.py:257-262) with
+  a gradient into x, q_proj and block_keys.
+* ``balance_loss(scores, remote_indices, remote_counts, base_blocks=...)`` is the load-balance loss over the
+  remote blocks with its gradient into the scores, and the blocks' slot counts; ``block_counts`` gives the
+  counts alone (for example to sum them over ranks first).
+
+The reference trains its router by distillation only; these operators have no counterpart there.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import kernels
+from ._lib import dtype_code, require_cuda
+
+CHECKPOINTS = (None, "mxfp8")
+
+
+def check_checkpoint(checkpoint: Optional[str]) -> Optional[str]:
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"unknown checkpoint {checkpoint!r}; expected one of {CHECKPOINTS}")
+    return checkpoint
+
+
+@dataclass
+class MXFP8Checkpoint:
+    """An 8-bit copy of a tensor: per 32 consecutive elements (row-major order) one power-of-two scale, the
+    smallest with max|x| <= 448 * scale over the block's finite elements, and e4m3 codes rounded to nearest
+    even (240 * 2^120 for the magnitudes that would round to 2^128).  NaN and infinities are kept as NaN."""
+
+    buffer: Tensor        # uint8: codes, padded to 16 bytes, then scale bytes
+    shape: torch.Size
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.buffer.numel()
+
+    @property
+    def codes(self) -> Tensor:
+        """The e4m3 codes, in the tensor's shape."""
+        return self.buffer[:self.shape.numel()].view(torch.float8_e4m3fn).view(self.shape)
+
+    @property
+    def scales(self) -> Tensor:
+        """One byte per block of 32 elements: the scale's exponent plus 127."""
+        return self.buffer[(self.shape.numel() + 15) // 16 * 16:]
+
+    def restore(self) -> Tensor:
+        """The values the copy stands for, in the tensor's shape and dtype (exact in fp32 and bf16)."""
+        return kernels.mxfp8_dequantize(self.buffer, self.shape, self.dtype)
+
+
+def checkpoint_mxfp8(x: Tensor) -> MXFP8Checkpoint:
+    """An 8-bit copy of ``x`` (fp32 or bf16 CUDA tensor, any shape); no gradient flows through it."""
+    return MXFP8Checkpoint(kernels.mxfp8_quantize(x.detach()), x.shape, x.dtype)
+
+
+class _RouterScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2d, q_proj, block_keys, keep):
+        scores, q16, rnorm, buf = kernels.router_scores_train(x2d, q_proj, block_keys, keep_mxfp8=keep)
+        ctx.keep, ctx.dtype = keep, x2d.dtype
+        ctx.save_for_backward(buf if keep else x2d, q_proj, block_keys, q16, rnorm)
+        return scores
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dscores):
+        kept, q_proj, block_keys, q16, rnorm = ctx.saved_tensors
+        one = q_proj.dtype == block_keys.dtype
+        dx, dw, dk = kernels.router_scores_bwd(dscores, None if ctx.keep else kept, kept if ctx.keep else None, q_proj,
+                                               block_keys, q16, rnorm, ctx.dtype,
+                                               grad_dtype=q_proj.dtype if one else torch.float32,
+                                               want=ctx.needs_input_grad[:3])
+        if not one:
+            dw = dw.to(q_proj.dtype) if dw is not None else None
+            dk = dk.to(block_keys.dtype) if dk is not None else None
+        return dx, dw, dk, None
+
+
+def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: Optional[str] = None) -> Tensor:
+    """``rms_norm(x q_proj^T) block_keys^T / 4`` per token, differentiable in all three: x [..., D] fp32 or
+    bf16, q_proj [16, D], block_keys [NB, 16] -> fp32 [..., NB].  With ``checkpoint="mxfp8"`` the backward
+    pass reads an 8-bit copy of x (it enters q_proj's gradient only)."""
+    check_checkpoint(checkpoint)
+    for t in (x, q_proj, block_keys):
+        dtype_code(t.dtype)
+    D = x.shape[-1] if x.dim() else 0
+    if q_proj.dim() != 2 or q_proj.shape[0] != 16 or q_proj.shape[1] != D or block_keys.dim() != 2 \
+            or block_keys.shape[1] != 16:
+        raise ValueError(f"shapes: x [..., D], q_proj [16, D], block_keys [NB, 16]; got x {tuple(x.shape)}, "
+                         f"q_proj {tuple(q_proj.shape)}, block_keys {tuple(block_keys.shape)}")
+    NB = block_keys.shape[0]
+    if D == 0 or D % 8 or not 1 <= NB <= 1024:
+        raise ValueError(f"the router takes widths that are multiples of 8 and 1 to 1024 blocks, got D {D}, NB {NB}")
+    require_cuda(x, q_proj, block_keys)
+    grad = torch.is_grad_enabled() and (x.requires_grad or q_proj.requires_grad or block_keys.requires_grad)
+    s = _RouterScores.apply(x.reshape(-1, D), q_proj, block_keys, grad and checkpoint is not None)
+    return s.view(*x.shape[:-1], NB)
+
+
+def _routes(remote_indices: Tensor, remote_counts: Tensor) -> Tuple[Tensor, Tensor]:
+    for t in (remote_indices, remote_counts):
+        if t.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"remote_indices and remote_counts are int32 or int64, got {t.dtype}")
+    if remote_indices.dim() < 1 or remote_indices.shape[:-1] != remote_counts.shape:
+        raise ValueError(f"shapes: remote_indices [..., capacity], remote_counts [...]; got "
+                         f"{tuple(remote_indices.shape)} and {tuple(remote_counts.shape)}")
+    M = remote_counts.numel()
+    return remote_indices.reshape(M, remote_indices.shape[-1]), remote_counts.reshape(M)
+
+
+def _valid(valid: Optional[Tensor], lead: torch.Size) -> Optional[Tensor]:
+    if valid is None:
+        return None
+    if valid.dtype != torch.bool or valid.shape != lead:
+        raise ValueError(f"valid is a bool tensor of shape {tuple(lead)}, got {valid.dtype} {tuple(valid.shape)}")
+    return valid.reshape(-1)
+
+
+def _check_blocks(num_blocks: int) -> int:
+    if not 1 <= int(num_blocks) <= 1024:
+        raise ValueError(f"1 to 1024 blocks, got {num_blocks}")
+    return int(num_blocks)
+
+
+def block_counts(remote_indices: Tensor, remote_counts: Tensor, num_blocks: int, *,
+                 valid: Optional[Tensor] = None) -> Tensor:
+    """int64 [num_blocks]: how many slots of the route lists name each block.  remote_indices
+    [..., capacity], of which row t's first remote_counts[t] count (ids outside [0, num_blocks) do not);
+    ``valid`` (bool [...]) leaves rows out, for example padding."""
+    NB = _check_blocks(num_blocks)
+    idx, cnt = _routes(remote_indices, remote_counts)
+    rows = _valid(valid, remote_counts.shape)
+    require_cuda(idx, cnt, rows)
+    _, counts, _ = kernels.balance_loss_fwd(None, idx, cnt, NB, 0, 1.0, rows)
+    return counts
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scores, idx, cnt, base, temperature, valid, counts_in):
+        loss, counts, state = kernels.balance_loss_fwd(scores, idx, cnt, scores.shape[1], base, temperature, valid,
+                                                       counts_in)
+        ctx.base, ctx.temperature = base, temperature
+        ctx.save_for_backward(scores, valid, state)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _dcounts):
+        scores, valid, state = ctx.saved_tensors
+        ds = kernels.balance_loss_bwd(scores, ctx.base, ctx.temperature, valid, state, dloss)
+        return ds, None, None, None, None, None, None
+
+
+def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts: Optional[Tensor], *,
+                 base_blocks: int, temperature: float = 1.0, valid: Optional[Tensor] = None,
+                 counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Load-balance loss of a routing and the blocks' slot counts.
+
+    scores [..., NB] are the router's scores (before the temperature), remote_indices [..., capacity] and
+    remote_counts [...] the routes chosen from them (``select_blocks``).  With p_t the softmax of
+    scores_t / temperature over the R = NB - base_blocks remote blocks, f_b block b's share of the slots and n
+    the number of rows, ``loss = R sum_b f_b (1/n) sum_t p_tb``: 1 for an even load, R when one block takes
+    everything.  The gradient reaches the scores through p only.
+
+    Rows whose ``valid`` is False or whose remote scores are all -inf are not counted and receive zeros.
+    ``counts`` (int64 [NB], :func:`block_counts` summed over ranks) replaces the lists' own counts; the
+    lists may be None then.  Returns (loss fp32 0-d, counts int64 [NB])."""
+    NB = _check_blocks(scores.shape[-1] if scores.dim() else 0)
+    if not 0 <= int(base_blocks) < NB:
+        raise ValueError(f"base_blocks must leave a remote block: 0 <= base_blocks < {NB}, got {base_blocks}")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not scores.is_floating_point():
+        raise TypeError(f"scores must be floating point, got {scores.dtype}")
+    lead = scores.shape[:-1]
+    idx = cnt = None
+    if counts is not None:
+        if counts.dtype != torch.int64 or counts.shape != (NB,):
+            raise ValueError(f"counts is an int64 tensor [{NB}], got {counts.dtype} {tuple(counts.shape)}")
+    else:
+        if remote_indices is None or remote_counts is None:
+            raise ValueError("remote_indices and remote_counts are needed unless counts are given")
+        idx, cnt = _routes(remote_indices, remote_counts)
+        if remote_counts.shape != lead:
+            raise ValueError(f"routes of {tuple(remote_counts.shape)} rows for scores of {tuple(lead)}")
+    rows = _valid(valid, lead)
+    require_cuda(scores, idx, cnt, rows, counts)
+    return _BalanceLoss.apply(scores.reshape(-1, NB).float(), idx, cnt, int(base_blocks), float(temperature), rows,
+                              counts)

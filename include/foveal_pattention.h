@@ -442,6 +442,70 @@ FP_API int fp_tokenformer_fwd(const void* x, int64_t M, int D_in, const void* k_
 FP_API int fp_transpose(const void* src, int64_t rows, int64_t cols, int dtype, void* dst, void* stream);
 
 /*
+ * 8-bit copies of activations (MXFP8), kept from a forward to its backward pass.  32 consecutive elements of
+ * the n (the last block may be shorter) share a scale 2^k, the smallest with max|x| <= 448 * 2^k over the
+ * block's finite elements, k in [-118, 120], stored as the byte k + 127; an element is the e4m3 code of
+ * x * 2^-k rounded to nearest even, the NaN code for a NaN or an infinity.  A dequantised value is exact in
+ * fp32 and bf16 (magnitudes of at least 248 * 2^120, which would round to 2^128, are held as 240 * 2^120).  codes: n bytes, 16-byte aligned; scales: ceil(n / 32) bytes.
+ */
+FP_API int fp_mxfp8_quantize(const void* x, int dtype, int64_t n, void* codes, void* scales, void* stream);
+FP_API int fp_mxfp8_dequantize(const void* codes, const void* scales, int dtype, int64_t n, void* y, void* stream);
+
+/*
+ * fp_swiglu_fwd that also leaves MXFP8 copies of g and u, and the backward that reads them: with g^, u^ the
+ * copies' values, dg = dout * u^ * silu'(g^), du = dout * silu(g^) and (optional, h may be NULL)
+ * h = silu(g^) * u^.  n elements; dout, dg, du and h in `dtype`; h of the forward equals fp_swiglu_fwd's.
+ */
+FP_API int fp_swiglu_fwd_mxfp8(const void* g, const void* u, int dtype, int64_t n, void* h, void* g_codes,
+                               void* g_scales, void* u_codes, void* u_scales, void* stream);
+FP_API int fp_swiglu_bwd_mxfp8(const void* dout, const void* g_codes, const void* g_scales, const void* u_codes,
+                               const void* u_scales, int dtype, int64_t n, void* dg, void* du, void* h,
+                               void* stream);
+
+/*
+ * fp_router_scores for training: the same scores, and what their gradient needs: q16 [M, 16] fp32 normalised
+ * queries, rnorm [M] fp32 factors 1 / rms(x . q_proj^T) and, unless codes and scales are NULL, the MXFP8 copy
+ * of x (M * D codes).
+ */
+FP_API int fp_router_scores_train(const void* x, const void* q_proj, const void* block_keys, int dtype, int64_t M,
+                                  int D, int NB, float* scores, float* q16, float* rnorm, void* codes, void* scales,
+                                  void* stream);
+
+/*
+ * Gradient of the router scores from dscores [M, NB] fp32:
+ *   a = dscores . K_16 / 4,  dq = rnorm * (a - q16 * mean(a * q16)),
+ *   dx = dq . q_proj,  dq_proj = dq^T . x,  dblock_keys = dscores^T . q16 / 4
+ * dx [M, D] in `dtype`, dq_proj [16, D] and dblock_keys [NB, 16] in grad_dtype; each may be NULL (not
+ * computed).  x may be NULL when codes and scales are given (its MXFP8 copy is read then, also when x is
+ * given) or dq_proj is not wanted.  The sums over tokens have a fixed order.
+ */
+FP_API size_t fp_router_scores_bwd_workspace_size(int64_t M, int D, int NB);
+FP_API int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes, const void* scales,
+                                const void* q_proj, const void* block_keys, const float* q16, const float* rnorm,
+                                int dtype, int64_t M, int D, int NB, void* dx, void* dq_proj, void* dblock_keys,
+                                int grad_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Load balance of the routed blocks.  R = NB - base_blocks remote blocks; a row is counted when valid[t] (NULL:
+ * all) and one of its remote scores is above -inf (a NaN counts and makes the result NaN); n rows are counted.
+ *   counts[b] = routed slots of block b over the valid rows: remote_indices [M, capacity], the first
+ *               remote_counts[t] of row t (at most capacity; ids outside [0, NB) are skipped)
+ *   p_t = softmax(scores[t, base:] / T),  f_b = counts[b] / sum(counts)   (0 when nothing was routed)
+ *   loss = R * sum_b f_b * (1/n) sum_t p_tb                               (0 when no row is counted)
+ * counts_in [NB] (optional) replaces the lists' own counts, for example summed over ranks.  loss and state
+ * [NB + 1] NULL: counts only (scores are not read).  fp_balance_loss_bwd: dscores from the state and the
+ * device scalar dloss; base columns and rows that are not counted receive zeros.  NB <= 1024.
+ */
+FP_API size_t fp_balance_workspace_size(int64_t M, int NB);
+FP_API int fp_balance_loss_fwd(const float* scores, int64_t M, int NB, int base_blocks, float temperature,
+                               const uint8_t* valid, const int32_t* remote_indices, const int32_t* remote_counts,
+                               int capacity, const int64_t* counts_in, int64_t* counts, float* loss, float* state,
+                               void* workspace, size_t workspace_bytes, void* stream);
+FP_API int fp_balance_loss_bwd(const float* scores, int64_t M, int NB, int base_blocks, float temperature,
+                               const uint8_t* valid, const float* state, const float* dloss, float* dscores,
+                               void* stream);
+
+/*
  * Measurement hook (no counterpart in the reference): for the calling host thread, the forward entry
  * points record events[i] (cudaEvent_t handles) on their stream at stage boundaries:
  *   fp_pattention_token_fwd:  0 start, 1 and 2 routed (scores, selection, block lists and H clears are
