@@ -10,78 +10,141 @@
 namespace fp {
 namespace {
 
-constexpr int kWarps = 8;
+// All four kernels stream: a thread takes kUnroll vectors of 16 bytes, a CTA's width apart, and issues all of
+// their loads before the first use.  HBM bound.
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;      // one tensor in
+constexpr int kUnroll2 = 2;     // two or three tensors in
+
+template <typename T, int U>
+__device__ __forceinline__ int64_t first_element() {
+  return ((int64_t)blockIdx.x * (kThreads * U) + threadIdx.x) * MxVec<T>::kV;
+}
+template <typename T>
+constexpr int kStep = kThreads * MxVec<T>::kV;
 
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kThreads)
 mxfp8_quantize_kernel(const T* __restrict__ x, int64_t n, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int lane = threadIdx.x & 31;
-  const int64_t nb = (n + kMxBlock - 1) / kMxBlock;
-  for (int64_t b = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); b < nb; b += (int64_t)gridDim.x * kWarps) {
-    const int64_t i = b * kMxBlock + lane;
-    int byte;
-    const uint8_t c = mx_quantize_lane(i < n ? to_f32(x[i]) : 0.f, byte);
-    if (i < n) codes[i] = c;
-    if (lane == 0) scales[b] = (uint8_t)byte;
+  using V = MxVec<T>;
+  const int64_t i = first_element<T, kUnroll>();
+  uint4 w[kUnroll];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) w[k] = V::load(x, i + k * kStep<T>, n);
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) V::quantize(w[k], i + k * kStep<T>, n, codes, scales);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+mxfp8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n,
+                        T* __restrict__ y) {
+  using V = MxVec<T>;
+  const int64_t i = first_element<T, kUnroll>();
+  typename V::Codes q[kUnroll];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) q[k] = V::load_codes(codes, scales, i + k * kStep<T>, n);
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) {
+    float v[V::kV];
+    V::values(q[k], v);
+    V::store(y, i + k * kStep<T>, n, v);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
-mxfp8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n,
-                        T* __restrict__ y) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    y[i] = mx_from_f32<T>(mx_value(codes[i], scales[i / kMxBlock]));
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kThreads)
 swiglu_fwd_mxfp8_kernel(const T* __restrict__ g, const T* __restrict__ u, int64_t n, T* __restrict__ h,
                         uint8_t* __restrict__ gc, uint8_t* __restrict__ gs, uint8_t* __restrict__ uc,
                         uint8_t* __restrict__ us) {
-  const int lane = threadIdx.x & 31;
-  const int64_t nb = (n + kMxBlock - 1) / kMxBlock;
-  for (int64_t b = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); b < nb; b += (int64_t)gridDim.x * kWarps) {
-    const int64_t i = b * kMxBlock + lane;
-    const float gv = i < n ? to_f32(g[i]) : 0.f, uv = i < n ? to_f32(u[i]) : 0.f;
-    int gb, ub;
-    const uint8_t cg = mx_quantize_lane(gv, gb), cu = mx_quantize_lane(uv, ub);
-    if (i < n) {
-      h[i] = mx_from_f32<T>(gv / (1.0f + expf(-gv)) * uv);
-      gc[i] = cg;
-      uc[i] = cu;
-    }
-    if (lane == 0) {
-      gs[b] = (uint8_t)gb;
-      us[b] = (uint8_t)ub;
-    }
+  using V = MxVec<T>;
+  const int64_t i0 = first_element<T, kUnroll2>();
+  uint4 gw[kUnroll2], uw[kUnroll2];
+#pragma unroll
+  for (int k = 0; k < kUnroll2; ++k) {
+    gw[k] = V::load(g, i0 + k * kStep<T>, n);
+    uw[k] = V::load(u, i0 + k * kStep<T>, n);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnroll2; ++k) {
+    const int64_t i = i0 + k * kStep<T>;
+    V::quantize(gw[k], i, n, gc, gs);
+    V::quantize(uw[k], i, n, uc, us);
+    float gv[V::kV], uv[V::kV];
+    V::unpack(gw[k], gv);
+    V::unpack(uw[k], uv);
+#pragma unroll
+    for (int e = 0; e < V::kV; ++e) gv[e] = gv[e] / (1.0f + expf(-gv[e])) * uv[e];  // as fp_swiglu_fwd
+    V::store(h, i, n, gv);
   }
 }
 
+// sigmoid(g).  For bf16 gradients the hardware exponential and reciprocal do: their error (about 2^-21 of
+// the value) is far below the gradients' own rounding (2^-9), and the exact forms made the backward kernel
+// issue bound.
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
+__device__ __forceinline__ float sigmoid_for(float g) {
+  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-g)));
+  return r;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
 swiglu_bwd_mxfp8_kernel(const T* __restrict__ dout, const uint8_t* __restrict__ gc, const uint8_t* __restrict__ gs,
                         const uint8_t* __restrict__ uc, const uint8_t* __restrict__ us, int64_t n,
                         T* __restrict__ dg, T* __restrict__ du, T* __restrict__ h) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const float d = to_f32(dout[i]);
-    const float gv = mx_value(gc[i], gs[i / kMxBlock]), uv = mx_value(uc[i], us[i / kMxBlock]);
-    const float sig = 1.0f / (1.0f + expf(-gv));
-    const float silu = gv * sig;
-    du[i] = mx_from_f32<T>(d * silu);
-    dg[i] = mx_from_f32<T>(d * uv * (sig * (1.0f + gv * (1.0f - sig))));
-    if (h) h[i] = mx_from_f32<T>(silu * uv);
+  using V = MxVec<T>;
+  const int64_t i0 = first_element<T, kUnroll2>();
+  uint4 dw[kUnroll2];
+  typename V::Codes gq[kUnroll2], uq[kUnroll2];
+#pragma unroll
+  for (int k = 0; k < kUnroll2; ++k) {
+    dw[k] = V::load(dout, i0 + k * kStep<T>, n);
+    gq[k] = V::load_codes(gc, gs, i0 + k * kStep<T>, n);
+    uq[k] = V::load_codes(uc, us, i0 + k * kStep<T>, n);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnroll2; ++k) {
+    const int64_t i = i0 + k * kStep<T>;
+    float d[V::kV], gv[V::kV], uv[V::kV];
+    V::unpack(dw[k], d);
+    V::values(gq[k], gv);
+    V::values(uq[k], uv);
+    float a[V::kV], b[V::kV], c[V::kV];
+#pragma unroll
+    for (int e = 0; e < V::kV; ++e) {
+      const float sig = sigmoid_for<T>(gv[e]);
+      const float silu = gv[e] * sig;
+      a[e] = d[e] * uv[e] * (sig * (1.0f + gv[e] * (1.0f - sig)));
+      b[e] = d[e] * silu;
+      c[e] = silu * uv[e];
+    }
+    V::store(dg, i, n, a);
+    V::store(du, i, n, b);
+    if (h) V::store(h, i, n, c);
   }
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-int grid_for(int64_t units, int64_t per_block, int sms) {
-  const int64_t want = (units + per_block - 1) / per_block;
-  return (int)(want < (int64_t)sms * 16 ? want : (int64_t)sms * 16);
+// CTAs of kThreads * unroll vectors for n elements; 0 when the grid would pass its limit.
+template <typename T>
+unsigned grid_for(int64_t n, int unroll) {
+  const int64_t per = (int64_t)kStep<T> * unroll, want = (n + per - 1) / per;
+  return want <= INT32_MAX ? (unsigned)want : 0u;
 }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? FP_OK : FP_ERR_CUDA; }
+
+// f(T{}) with the element type of `dtype`, once the current device is known to run these kernels.
+template <typename F>
+int by_type(int dtype, F f) {
+  int sms;
+  if (const int rc = device_info(sms)) return rc;
+  return dtype == FP_DTYPE_BF16 ? f(__nv_bfloat16{}) : f(float{});
+}
 
 bool known(int dtype) { return dtype == FP_DTYPE_F32 || dtype == FP_DTYPE_BF16; }
 
@@ -97,15 +160,14 @@ int fp_mxfp8_quantize(const void* x, int dtype, int64_t n, void* codes, void* sc
   if (!known(dtype)) return FP_ERR_UNSUPPORTED;
   if (n == 0) return FP_OK;
   if (!x || !codes || !scales || !al16(x) || !al16(codes)) return FP_ERR_INVALID_ARG;
-  int sms;
-  if (const int rc = device_info(sms)) return rc;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int grid = grid_for(n, kWarps * 32, sms);
-  if (dtype == FP_DTYPE_BF16)
-    mxfp8_quantize_kernel<<<grid, kWarps * 32, 0, st>>>((const __nv_bfloat16*)x, n, (uint8_t*)codes, (uint8_t*)scales);
-  else
-    mxfp8_quantize_kernel<<<grid, kWarps * 32, 0, st>>>((const float*)x, n, (uint8_t*)codes, (uint8_t*)scales);
-  return launched();
+  return by_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const unsigned grid = grid_for<T>(n, kUnroll);
+    if (!grid) return FP_ERR_UNSUPPORTED;
+    mxfp8_quantize_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T*)x, n, (uint8_t*)codes,
+                                                                         (uint8_t*)scales);
+    return launched();
+  });
 }
 
 int fp_mxfp8_dequantize(const void* codes, const void* scales, int dtype, int64_t n, void* y, void* stream) {
@@ -113,16 +175,14 @@ int fp_mxfp8_dequantize(const void* codes, const void* scales, int dtype, int64_
   if (!known(dtype)) return FP_ERR_UNSUPPORTED;
   if (n == 0) return FP_OK;
   if (!y || !codes || !scales || !al16(y) || !al16(codes)) return FP_ERR_INVALID_ARG;
-  int sms;
-  if (const int rc = device_info(sms)) return rc;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int grid = grid_for(n, kWarps * 32, sms);
-  if (dtype == FP_DTYPE_BF16)
-    mxfp8_dequantize_kernel<<<grid, kWarps * 32, 0, st>>>((const uint8_t*)codes, (const uint8_t*)scales, n,
-                                                         (__nv_bfloat16*)y);
-  else
-    mxfp8_dequantize_kernel<<<grid, kWarps * 32, 0, st>>>((const uint8_t*)codes, (const uint8_t*)scales, n, (float*)y);
-  return launched();
+  return by_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const unsigned grid = grid_for<T>(n, kUnroll);
+    if (!grid) return FP_ERR_UNSUPPORTED;
+    mxfp8_dequantize_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const uint8_t*)codes,
+                                                                           (const uint8_t*)scales, n, (T*)y);
+    return launched();
+  });
 }
 
 int fp_swiglu_fwd_mxfp8(const void* g, const void* u, int dtype, int64_t n, void* h, void* g_codes, void* g_scales,
@@ -132,19 +192,15 @@ int fp_swiglu_fwd_mxfp8(const void* g, const void* u, int dtype, int64_t n, void
   if (n == 0) return FP_OK;
   if (!g || !u || !h || !g_codes || !g_scales || !u_codes || !u_scales) return FP_ERR_INVALID_ARG;
   if (!al16(g) || !al16(u) || !al16(h) || !al16(g_codes) || !al16(u_codes)) return FP_ERR_INVALID_ARG;
-  int sms;
-  if (const int rc = device_info(sms)) return rc;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int grid = grid_for(n, kWarps * 32, sms);
-  if (dtype == FP_DTYPE_BF16)
-    swiglu_fwd_mxfp8_kernel<<<grid, kWarps * 32, 0, st>>>(
-        (const __nv_bfloat16*)g, (const __nv_bfloat16*)u, n, (__nv_bfloat16*)h, (uint8_t*)g_codes, (uint8_t*)g_scales,
-        (uint8_t*)u_codes, (uint8_t*)u_scales);
-  else
-    swiglu_fwd_mxfp8_kernel<<<grid, kWarps * 32, 0, st>>>((const float*)g, (const float*)u, n, (float*)h,
-                                                         (uint8_t*)g_codes, (uint8_t*)g_scales, (uint8_t*)u_codes,
-                                                         (uint8_t*)u_scales);
-  return launched();
+  return by_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const unsigned grid = grid_for<T>(n, kUnroll2);
+    if (!grid) return FP_ERR_UNSUPPORTED;
+    swiglu_fwd_mxfp8_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>(
+        (const T*)g, (const T*)u, n, (T*)h, (uint8_t*)g_codes, (uint8_t*)g_scales, (uint8_t*)u_codes,
+        (uint8_t*)u_scales);
+    return launched();
+  });
 }
 
 int fp_swiglu_bwd_mxfp8(const void* dout, const void* g_codes, const void* g_scales, const void* u_codes,
@@ -154,19 +210,15 @@ int fp_swiglu_bwd_mxfp8(const void* dout, const void* g_codes, const void* g_sca
   if (n == 0) return FP_OK;
   if (!dout || !dg || !du || !g_codes || !g_scales || !u_codes || !u_scales) return FP_ERR_INVALID_ARG;
   if (!al16(dout) || !al16(dg) || !al16(du) || !al16(h) || !al16(g_codes) || !al16(u_codes)) return FP_ERR_INVALID_ARG;
-  int sms;
-  if (const int rc = device_info(sms)) return rc;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int grid = grid_for(n, kWarps * 32, sms);
-  if (dtype == FP_DTYPE_BF16)
-    swiglu_bwd_mxfp8_kernel<<<grid, kWarps * 32, 0, st>>>(
-        (const __nv_bfloat16*)dout, (const uint8_t*)g_codes, (const uint8_t*)g_scales, (const uint8_t*)u_codes,
-        (const uint8_t*)u_scales, n, (__nv_bfloat16*)dg, (__nv_bfloat16*)du, (__nv_bfloat16*)h);
-  else
-    swiglu_bwd_mxfp8_kernel<<<grid, kWarps * 32, 0, st>>>(
-        (const float*)dout, (const uint8_t*)g_codes, (const uint8_t*)g_scales, (const uint8_t*)u_codes,
-        (const uint8_t*)u_scales, n, (float*)dg, (float*)du, (float*)h);
-  return launched();
+  return by_type(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const unsigned grid = grid_for<T>(n, kUnroll2);
+    if (!grid) return FP_ERR_UNSUPPORTED;
+    swiglu_bwd_mxfp8_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>(
+        (const T*)dout, (const uint8_t*)g_codes, (const uint8_t*)g_scales, (const uint8_t*)u_codes,
+        (const uint8_t*)u_scales, n, (T*)dg, (T*)du, (T*)h);
+    return launched();
+  });
 }
 
 }  // extern "C"

@@ -35,136 +35,542 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 
 // ------------------------------------------------------------------ gradient of the scores
-// dq, one warp per token.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// Three launches.  (1) One pass over dS: dq of every token and partial sums of dK.  (2) One pass over x: dx and
+// partial sums of dWq.  (3) The partial sums, in a fixed order.  The products are 16 wide on one side, so the
+// passes are bound by memory once they run on tensor cores; a tile of 128 rows (tcgen05) would be filled to
+// an eighth, mma.sync fits: the 16 router dimensions are its m (pass 1) and its k or two n-tiles (pass 2).
+//
+// Precision.  Pass 1 multiplies fp32 values as tf32 pieces, v = hi + lo (the rest is below 2^-22 of v):
+// hi hi + hi lo + lo hi, fp32 accumulators.  Pass 2 with bf16 x holds dq as two bf16 pieces (rest below
+// 2^-17 of dq, against 2^-9 for the bf16 gradients), x and Wq are exact.  fp32 x stays on the FMA units.
+//
+// Fragment coordinates below: lane = 4 g + t, g = 0..7, t = 0..3.
+
+__device__ __forceinline__ uint32_t tf32_of(float v) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ void tf32_split(float v, uint32_t& hi, uint32_t& lo) {
+  hi = tf32_of(v);
+  lo = tf32_of(v - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Four columns of one row of dS, zeros outside.
+__device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, int64_t M, int b, int NB, bool vec) {
+  if (t >= M || b >= NB) return make_float4(0.f, 0.f, 0.f, 0.f);
+  const float* p = ds + t * NB + b;
+  if (vec) return __ldg(reinterpret_cast<const float4*>(p));
+  return make_float4(p[0], b + 1 < NB ? p[1] : 0.f, b + 2 < NB ? p[2] : 0.f, b + 3 < NB ? p[3] : 0.f);
+}
+
+constexpr int kDqWarps = 4;
+constexpr int kDqTokens = 16 * kDqWarps;  // tokens of a CTA's tile
+constexpr int kDqMaxCtas = 296;
+
+// Pass 1.  Phase A, 16 tokens to a warp: a^T[j, tok] = K^T[j, b] dS^T[b, tok], then dq.  Phase B, a share of
+// the blocks (kG groups of 32) to a warp, over the CTA's 64 tokens (rows just read, from L1): dK^T[j, b] =
+// n^T[j, tok] dS[tok, b], kept in registers over all of the CTA's tiles.  The order of b within a product and
+// the columns of a tile are permuted so that a lane's elements are 16 contiguous bytes.
+// dq: kPacked, per tile of 16 tokens the two bf16 pieces as pass 2's fragments ([tile][hi, lo][lane] uint4);
+// otherwise fp32 [M, 16].
+template <typename T, int kG, bool kPacked>
+__global__ void __launch_bounds__(kDqWarps * 32)
 router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const float* __restrict__ q16,
-                 const float* __restrict__ rnorm, int64_t M, int NB, float* __restrict__ dq) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < M; t += (int64_t)gridDim.x * 8) {
-    float a[kIdx] = {};
-    for (int b = lane; b < NB; b += 32) {
-      const float s = ds[t * NB + b];
-#pragma unroll
-      for (int j = 0; j < kIdx; ++j) a[j] = fmaf(s, to_f32(k16[b * kIdx + j]), a[j]);
+                 const float* __restrict__ rnorm, int64_t M, int NB, void* __restrict__ dq_out,
+                 float* __restrict__ dk_part) {
+  extern __shared__ float4 sk[];  // [ceil(NB / 16)][2][32]: K as phase A's fragments
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int nk = (NB + 15) / 16;
+  const bool vec = (NB & 3) == 0;
+  if (dq_out) {
+    for (int i = threadIdx.x; i < nk * 64; i += blockDim.x) {
+      const int l = i & 31, s = (i >> 5) & 1, b = (i >> 6) * 16 + 4 * (l & 3) + 2 * s, j = l >> 2;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (b < NB) {
+        v.x = to_f32(k16[b * kIdx + j]);
+        v.y = to_f32(k16[b * kIdx + j + 8]);
+      }
+      if (b + 1 < NB) {
+        v.z = to_f32(k16[(b + 1) * kIdx + j]);
+        v.w = to_f32(k16[(b + 1) * kIdx + j + 8]);
+      }
+      sk[i] = v;
     }
-    float dot = 0.f, n[kIdx];
+    __syncthreads();
+  }
+  float dk[kG][4][4];
 #pragma unroll
-    for (int j = 0; j < kIdx; ++j) {
-      a[j] = warp_sum(a[j]) * 0.25f;
-      n[j] = q16[t * kIdx + j];
-      dot = fmaf(a[j], n[j], dot);
+  for (int i = 0; i < kG; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dk[i][k][e] = 0.f;
+
+  for (int64_t base = (int64_t)blockIdx.x * kDqTokens; base < M; base += (int64_t)gridDim.x * kDqTokens) {
+    const int64_t tok0 = base + 16 * warp;
+    if (dq_out && tok0 < M) {
+      float c[2][4] = {};
+#pragma unroll 2
+      for (int k = 0; k < nk; ++k) {
+        float4 v[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) v[n] = ds4(ds, tok0 + 8 * n + g, M, 16 * k + 4 * t, NB, vec);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const float4 kv = sk[(k * 2 + s) * 32 + lane];
+          const float kf[4] = {kv.x, kv.y, kv.z, kv.w};
+          uint32_t kh[4], kl[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) tf32_split(kf[e], kh[e], kl[e]);
+            else kh[e] = __float_as_uint(kf[e]);  // a bf16 value is a tf32 value
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t h0, l0, h1, l1;
+            tf32_split(s ? v[n].z : v[n].x, h0, l0);
+            tf32_split(s ? v[n].w : v[n].y, h1, l1);
+            mma_tf32(c[n], kh, l0, l1);
+            if constexpr (sizeof(T) == 4) mma_tf32(c[n], kl, h0, h1);
+            mma_tf32(c[n], kh, h0, h1);
+          }
+        }
+      }
+      // c[n]: token 8 n + 2 t (+1: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
+      uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float d[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t tok = tok0 + 8 * n + 2 * t + e;
+          const bool in = tok < M;
+          const float n0 = in ? q16[tok * kIdx + g] : 0.f, n1 = in ? q16[tok * kIdx + g + 8] : 0.f;
+          const float a0 = c[n][e] * 0.25f, a1 = c[n][2 + e] * 0.25f;
+          float dot = a0 * n0 + a1 * n1;
+          dot += __shfl_xor_sync(0xffffffffu, dot, 4);
+          dot += __shfl_xor_sync(0xffffffffu, dot, 8);
+          dot += __shfl_xor_sync(0xffffffffu, dot, 16);
+          dot *= 1.0f / kIdx;
+          const float r = in ? rnorm[tok] : 0.f;
+          d[0][e] = in ? r * (a0 - n0 * dot) : 0.f;
+          d[1][e] = in ? r * (a1 - n1 * dot) : 0.f;
+          if constexpr (!kPacked) {
+            if (in) {
+              float* o = reinterpret_cast<float*>(dq_out) + tok * kIdx + g;
+              o[0] = d[0][e];
+              o[8] = d[1][e];
+            }
+          }
+        }
+        if constexpr (kPacked) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t h = pack_bf16(d[j][0], d[j][1]);
+            hi[n][j] = h;
+            lo[n][j] = pack_bf16(d[j][0] - __uint_as_float(h << 16), d[j][1] - __uint_as_float(h & 0xFFFF0000u));
+          }
+        }
+      }
+      if constexpr (kPacked) {
+        uint4* o = reinterpret_cast<uint4*>(dq_out) + (tok0 / 16) * 64 + lane;
+        o[0] = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
+        o[32] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
+      }
     }
-    dot *= 1.0f / kIdx;
-    const float r = rnorm[t];
+    if (dk_part) {
+      const int64_t end = min(base + kDqTokens, M);
+      for (int64_t s0 = base; s0 < end; s0 += 8) {
+        const int64_t ta = s0 + t, tb = s0 + t + 4;
+        uint32_t nh[4], nl[4];
+        const float n4[4] = {ta < M ? q16[ta * kIdx + g] : 0.f, ta < M ? q16[ta * kIdx + g + 8] : 0.f,
+                             tb < M ? q16[tb * kIdx + g] : 0.f, tb < M ? q16[tb * kIdx + g + 8] : 0.f};
 #pragma unroll
-    for (int j = 0; j < kIdx; ++j)
-      if (lane == j) dq[t * kIdx + j] = r * (a[j] - n[j] * dot);
+        for (int e = 0; e < 4; ++e) tf32_split(n4[e], nh[e], nl[e]);
+#pragma unroll
+        for (int i = 0; i < kG; ++i) {
+          const int b = 32 * (warp + kDqWarps * i) + 4 * g;
+          const float4 va = ds4(ds, ta, M, b, NB, vec), vb = ds4(ds, tb, M, b, NB, vec);
+          const float fa[4] = {va.x, va.y, va.z, va.w}, fb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t h0, l0, h1, l1;
+            tf32_split(fa[k], h0, l0);
+            tf32_split(fb[k], h1, l1);
+            mma_tf32(dk[i][k], nh, l0, l1);
+            mma_tf32(dk[i][k], nl, h0, h1);
+            mma_tf32(dk[i][k], nh, h0, h1);
+          }
+        }
+      }
+    }
+  }
+  if (dk_part) {  // dk[i][k]: b = 32 (..) + 8 t + k (+4: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
+    float* o = dk_part + (int64_t)blockIdx.x * NB * kIdx;
+#pragma unroll
+    for (int i = 0; i < kG; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int b = 32 * (warp + kDqWarps * i) + 8 * t + 4 * (e & 1) + k;
+          if (b < NB) o[b * kIdx + g + 8 * (e >> 1)] = dk[i][k][e] * 0.25f;
+        }
   }
 }
 
-// Partial sums over the token range of blockIdx.y: dK, one thread per element.
-__global__ void __launch_bounds__(256)
-router_dk_kernel(const float* __restrict__ ds, const float* __restrict__ q16, int64_t M, int NB, int64_t chunk,
-                 float* __restrict__ part) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= NB * kIdx) return;
-  const int b = i / kIdx, j = i % kIdx;
-  const int64_t t0 = blockIdx.y * chunk, t1 = min(t0 + chunk, M);
-  float s = 0.f;
-  for (int64_t t = t0; t < t1; ++t) s = fmaf(ds[t * NB + b], q16[t * kIdx + j], s);
-  part[(int64_t)blockIdx.y * NB * kIdx + i] = s * 0.25f;
-}
+// Pass 2, bf16.  A warp owns 64 columns and steps through its CTA's tokens 16 at a time: the lane's four 16-byte
+// pieces of x (tokens 2t, 2t+1, 2t+8, 2t+9, columns 8g..) become the dWq product's A operand by permuting
+// halfwords of two tokens' words, without shared memory; dWq^T[d, j] stays in 32 registers over all tokens.
+// dx[tok, d] = dq Wq takes dq's fragments transposed (movmatrix) and Wq's from registers, its columns permuted
+// so that a lane stores 16 contiguous bytes.  wd warps (1, 2, 4) lie along the columns, 8 / wd along tokens;
+// the token groups' dWq are joined in shared memory, in order.
+constexpr int kXWarps = 8;
 
-// dWq over the token range of blockIdx.y, one thread per column; x from its 8-bit copy when codes are given.
-template <typename T>
-__global__ void __launch_bounds__(256)
-router_dw_kernel(const T* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                 const float* __restrict__ dq, int64_t M, int D, int64_t chunk, float* __restrict__ part) {
-  const int d = blockIdx.x * blockDim.x + threadIdx.x;
-  if (d >= D) return;
-  const int64_t t0 = blockIdx.y * chunk, t1 = min(t0 + chunk, M);
-  float acc[kIdx] = {};
-  for (int64_t t = t0; t < t1; ++t) {
-    const int64_t i = t * D + d;
-    const float v = codes ? mx_value(codes[i], scales[i / kMxBlock]) : to_f32(x[i]);
+template <bool kCodes>
+struct XRows {
+  uint4 r[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__ codes,
+                                       const uint8_t* __restrict__ scales, int64_t tok0, int64_t M, int D, int d, int t) {
+    uint2 c[4];
+    uint32_t byte[4];
 #pragma unroll
-    for (int j = 0; j < kIdx; ++j) acc[j] = fmaf(dq[t * kIdx + j], v, acc[j]);
+    for (int k = 0; k < 4; ++k) {
+      const int64_t tok = tok0 + 2 * t + (k & 1) + 8 * (k >> 1);
+      const bool in = tok < M && d < D;
+      const int64_t i = tok * D + d;
+      if constexpr (kCodes) {
+        c[k] = in ? __ldg(reinterpret_cast<const uint2*>(codes + i)) : make_uint2(0, 0);
+        byte[k] = in ? __ldg(scales + i / kMxBlock) : 127u;
+      } else {
+        r[k] = in ? __ldg(reinterpret_cast<const uint4*>(x + i)) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    if constexpr (kCodes) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float s = mx_scale((int)byte[k]);
+        const float2 a = mx_unpack2((uint16_t)c[k].x), b = mx_unpack2((uint16_t)(c[k].x >> 16));
+        const float2 e = mx_unpack2((uint16_t)c[k].y), f = mx_unpack2((uint16_t)(c[k].y >> 16));
+        r[k] = make_uint4(pack_bf16(a.x * s, a.y * s), pack_bf16(b.x * s, b.y * s), pack_bf16(e.x * s, e.y * s),
+                          pack_bf16(f.x * s, f.y * s));
+      }
+    }
   }
-#pragma unroll
-  for (int j = 0; j < kIdx; ++j) part[((int64_t)blockIdx.y * kIdx + j) * D + d] = acc[j];
-}
+};
 
-template <typename T>
-__global__ void __launch_bounds__(256)
-router_dx_kernel(const float* __restrict__ dq, const T* __restrict__ wq, int64_t M, int D, T* __restrict__ dx) {
-  const int64_t n = M * D;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t t = i / D;
-    const int d = (int)(i - t * D);
+template <bool kCodes>
+__global__ void __launch_bounds__(kXWarps * 32, 2)
+router_x_kernel(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__ codes,
+                const uint8_t* __restrict__ scales, const uint4* __restrict__ dq, const __nv_bfloat16* __restrict__ wq,
+                int64_t M, int D, int wd, int64_t tiles_per_cta, __nv_bfloat16* __restrict__ dx,
+                float* __restrict__ dw_part) {
+  __shared__ float red[kXWarps * 64 * kIdx];  // [token group][j][wd * 64]
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int dw = warp % wd, tw = warp / wd, ntw = kXWarps / wd;
+  const int d0 = (blockIdx.x * wd + dw) * 64, dl = d0 + 8 * g;
+  uint32_t wb[8][2];
+  if (dx) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = d0 + 32 * (i >> 2) + 8 * (g >> 1) + 2 * (i & 3) + (g & 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = 2 * t + 8 * h;
+        const uint32_t a = d < D ? (uint32_t)__bfloat16_as_ushort(wq[(int64_t)j * D + d]) : 0u;
+        const uint32_t b = d < D ? (uint32_t)__bfloat16_as_ushort(wq[(int64_t)(j + 1) * D + d]) : 0u;
+        wb[i][h] = a | (b << 16);
+      }
+    }
+  }
+  float acc[4][2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+  const int64_t tiles = (M + 15) / 16;
+  const int64_t tile1 = min((int64_t)(blockIdx.y + 1) * tiles_per_cta, tiles);
+  griddep_wait();
+  for (int64_t tile = (int64_t)blockIdx.y * tiles_per_cta + tw; tile < tile1; tile += ntw) {
+    XRows<kCodes> xr;
+    if (dw_part) xr.load(x, codes, scales, tile * 16, M, D, dl, t);
+    const uint4 h4 = __ldg(dq + tile * 64 + lane), l4 = __ldg(dq + tile * 64 + 32 + lane);
+    if (dx) {
+      const uint32_t ah[4] = {transpose8x8(h4.x), transpose8x8(h4.z), transpose8x8(h4.y), transpose8x8(h4.w)};
+      const uint32_t al[4] = {transpose8x8(l4.x), transpose8x8(l4.z), transpose8x8(l4.y), transpose8x8(l4.w)};
+      const int64_t ra = tile * 16 + g, rb = ra + 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t oa[4], ob[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_bf16(c, al[0], al[1], al[2], al[3], wb[4 * h + i][0], wb[4 * h + i][1]);
+          mma_bf16(c, ah[0], ah[1], ah[2], ah[3], wb[4 * h + i][0], wb[4 * h + i][1]);
+          oa[i] = pack_bf16(c[0], c[1]);
+          ob[i] = pack_bf16(c[2], c[3]);
+        }
+        const int d = d0 + 32 * h + 8 * t;
+        if (d < D) {
+          if (ra < M) *reinterpret_cast<uint4*>(dx + ra * D + d) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+          if (rb < M) *reinterpret_cast<uint4*>(dx + rb * D + d) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+        }
+      }
+    }
+    if (dw_part) {
+      const uint32_t w0[4] = {xr.r[0].x, xr.r[0].y, xr.r[0].z, xr.r[0].w}, w1[4] = {xr.r[1].x, xr.r[1].y, xr.r[1].z, xr.r[1].w};
+      const uint32_t w2[4] = {xr.r[2].x, xr.r[2].y, xr.r[2].z, xr.r[2].w}, w3[4] = {xr.r[3].x, xr.r[3].y, xr.r[3].z, xr.r[3].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a0 = __byte_perm(w0[i], w1[i], 0x5410), a1 = __byte_perm(w0[i], w1[i], 0x7632);
+        const uint32_t a2 = __byte_perm(w2[i], w3[i], 0x5410), a3 = __byte_perm(w2[i], w3[i], 0x7632);
+        mma_bf16(acc[i][0], a0, a1, a2, a3, l4.x, l4.z);
+        mma_bf16(acc[i][1], a0, a1, a2, a3, l4.y, l4.w);
+        mma_bf16(acc[i][0], a0, a1, a2, a3, h4.x, h4.z);
+        mma_bf16(acc[i][1], a0, a1, a2, a3, h4.y, h4.w);
+      }
+    }
+  }
+  if (!dw_part) return;
+  // acc[i][j]: column 8 g + 2 i (elements 0, 1) and + 1 (2, 3), dimension 8 j + 2 t (+1: odd element)
+  const int width = wd * 64;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(tw * kIdx + 8 * j + 2 * t + (e & 1)) * width + dw * 64 + 8 * g + 2 * i + (e >> 1)] = acc[i][j][e];
+  __syncthreads();
+  float* part = dw_part + (int64_t)blockIdx.y * kIdx * D;
+  const int db = blockIdx.x * width;
+  for (int i = threadIdx.x; i < kIdx * width; i += blockDim.x) {
+    const int j = i / width, d = i % width;
     float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < kIdx; ++j) s = fmaf(dq[t * kIdx + j], to_f32(wq[(int64_t)j * D + d]), s);
-    dx[i] = mx_from_f32<T>(s);
+    for (int k = 0; k < ntw; ++k) s += red[k * kIdx * width + i];
+    if (db + d < D) part[(int64_t)j * D + db + d] = s;
   }
 }
 
-// out[i] = sum over the partials in their order.
-template <typename T>
-__global__ void __launch_bounds__(256)
-sum_partials_kernel(const float* __restrict__ part, int parts, int64_t n, T* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int p = 0; p < parts; ++p) s += part[p * n + i];
-  out[i] = mx_from_f32<T>(s);
+// Pass 2, fp32, on the FMA units (32 per element): a thread owns 4 columns (their Wq and dWq in registers),
+// dq of 32 tokens at a time in shared memory; tx threads (32, 64, 128) lie along the columns, 128 / tx along
+// tokens.
+constexpr int kFThreads = 128;
+constexpr int kFTokens = 32;
+
+template <bool kCodes>
+__global__ void __launch_bounds__(kFThreads, 3)
+router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                    const float* __restrict__ dq, const float* __restrict__ wq, int64_t M, int D, int tx,
+                    int64_t tokens_per_cta, float* __restrict__ dx, float* __restrict__ dw_part) {
+  __shared__ float4 sq[kFTokens * 4];
+  __shared__ float red[kFThreads * 4 * kIdx];
+  griddep_launch_dependents();
+  const int lane = threadIdx.x % tx, ty = threadIdx.x / tx, nty = kFThreads / tx;
+  const int d = (blockIdx.x * tx + lane) * 4;
+  const bool in = d < D;
+  float w[kIdx][4], acc[kIdx][4];
+#pragma unroll
+  for (int j = 0; j < kIdx; ++j) {
+    const float4 v = in && dx ? __ldg(reinterpret_cast<const float4*>(wq + (int64_t)j * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+  }
+  const int64_t t1 = min((int64_t)(blockIdx.y + 1) * tokens_per_cta, M);
+  griddep_wait();
+  for (int64_t t0 = (int64_t)blockIdx.y * tokens_per_cta; t0 < t1; t0 += kFTokens) {
+    const int n = (int)min((int64_t)kFTokens, t1 - t0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * 4; i += kFThreads) sq[i] = __ldg(reinterpret_cast<const float4*>(dq + t0 * kIdx) + i);
+    __syncthreads();
+    if (!in) continue;
+#pragma unroll 2
+    for (int k = ty; k < n; k += nty) {
+      const int64_t i = (t0 + k) * D + d;
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (dw_part) {
+        if constexpr (kCodes) {
+          const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes + i));
+          const float s = mx_scale((int)__ldg(scales + i / kMxBlock));
+          const float2 a = mx_unpack2((uint16_t)c), b = mx_unpack2((uint16_t)(c >> 16));
+          v[0] = a.x * s; v[1] = a.y * s; v[2] = b.x * s; v[3] = b.y * s;
+        } else {
+          const float4 q = __ldg(reinterpret_cast<const float4*>(x + i));
+          v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        }
+      }
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) {
+        const float4 q4 = sq[k * 4 + jj];
+        const float q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[4 * jj + j][e] = fmaf(q[j], v[e], acc[4 * jj + j][e]);
+            o[e] = fmaf(q[j], w[4 * jj + j][e], o[e]);
+          }
+      }
+      if (dx) *reinterpret_cast<float4*>(dx + i) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+  }
+  if (!dw_part) return;
+  const int width = tx * 4;
+#pragma unroll
+  for (int j = 0; j < kIdx; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[(ty * kIdx + j) * width + lane * 4 + e] = acc[j][e];
+  __syncthreads();
+  float* part = dw_part + (int64_t)blockIdx.y * kIdx * D;
+  const int db = blockIdx.x * width;
+  for (int i = threadIdx.x; i < kIdx * width; i += kFThreads) {
+    const int j = i / width, c = i % width;
+    float s = 0.f;
+    for (int k = 0; k < nty; ++k) s += red[k * kIdx * width + i];
+    if (db + c < D) part[(int64_t)j * D + db + c] = s;
+  }
 }
 
+// Pass 3: out[i] = sum over the partials, 8 interleaved sums joined in order; dWq (n1 elements), then dK (n2).
+template <typename T>
+__global__ void __launch_bounds__(256)
+sum_partials_kernel(const float* __restrict__ p1, int parts1, int64_t n1, T* __restrict__ o1,
+                    const float* __restrict__ p2, int parts2, int64_t n2, T* __restrict__ o2) {
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int64_t blocks1 = (n1 + 31) / 32;
+  const bool first = blockIdx.x < blocks1;
+  const float* p = first ? p1 : p2;
+  const int64_t n = first ? n1 : n2, i = (first ? blockIdx.x : blockIdx.x - blocks1) * 32 + lane;
+  const int parts = first ? parts1 : parts2;
+  griddep_wait();
+  float v = 0.f;
+  if (i < n) {
+#pragma unroll 4
+    for (int k = row; k < parts; k += 8) v += p[k * n + i];
+  }
+  s[row][lane] = v;
+  __syncthreads();
+  if (row == 0 && i < n) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += s[k][lane];
+    (first ? o1 : o2)[i] = mx_from_f32<T>(v);
+  }
+}
+
+// Launch shapes and workspace of the three passes: about two CTAs of pass 2 to an SM (three for fp32), and no
+// more partial sums than that.
 struct BwdPlan {
-  int64_t chunk;  // tokens per partial sum
-  int parts;
+  int dq_ctas, wide, col_ctas, parts;
+  int64_t per_cta;  // pass 2: tiles of 16 tokens (bf16) or tokens (fp32)
   size_t dq, dw, dk, total;
 };
-BwdPlan bwd_plan(int64_t M, int D, int NB) {
+BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
   BwdPlan p{};
-  p.chunk = std::max<int64_t>(64, (M + 31) / 32);
-  p.parts = (int)((M + p.chunk - 1) / p.chunk);
+  p.dq_ctas = (int)std::min<int64_t>((M + kDqTokens - 1) / kDqTokens, kDqMaxCtas);
+  int64_t units;
+  if (dtype == FP_DTYPE_BF16) {
+    p.wide = D <= 64 ? 1 : D <= 128 ? 2 : 4;
+    p.col_ctas = (D + 64 * p.wide - 1) / (64 * p.wide);
+    units = (M + 15) / 16;
+    p.per_cta = std::max<int64_t>((units + std::max(296 / p.col_ctas, 1) - 1) / std::max(296 / p.col_ctas, 1),
+                                  2 * kXWarps / p.wide);
+  } else {
+    p.wide = D <= 128 ? 32 : D <= 256 ? 64 : 128;
+    p.col_ctas = (D + 4 * p.wide - 1) / (4 * p.wide);
+    units = M;
+    const int64_t want = std::max(444 / p.col_ctas, 1);
+    p.per_cta = std::max<int64_t>((units + want - 1) / want, kFTokens);
+  }
+  p.parts = (int)((units + p.per_cta - 1) / p.per_cta);
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p.dq = 0;
-  p.dw = p.dq + up((size_t)M * kIdx * 4);
+  p.dw = p.dq + up((size_t)((M + 15) / 16) * 1024);
   p.dk = p.dw + up((size_t)p.parts * kIdx * D * 4);
-  p.total = p.dk + up((size_t)p.parts * kIdx * NB * 4);
+  p.total = p.dk + up((size_t)p.dq_ctas * kIdx * NB * 4);
   return p;
+}
+
+template <typename T, int kG>
+int launch_dq(const BwdPlan& p, const float* ds, const T* k16, const float* q16, const float* rnorm, int64_t M, int NB,
+              void* dq, float* pk, cudaStream_t st) {
+  const auto kern = router_dq_kernel<T, kG, sizeof(T) == 2>;
+  const size_t smem = dq ? (size_t)((NB + 15) / 16) * 1024 : 0;  // at most 64 KB
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return FP_ERR_CUDA;
+  kern<<<p.dq_ctas, kDqWarps * 32, smem, st>>>(ds, k16, q16, rnorm, M, NB, dq, pk);
+  return launched();
 }
 
 template <typename T>
 int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t* scales, const T* wq, const T* k16,
                const float* q16, const float* rnorm, int64_t M, int D, int NB, T* dx, void* dwq, void* dk16,
-               int grad_dtype, char* ws, int sms, cudaStream_t st) {
-  const BwdPlan p = bwd_plan(M, D, NB);
-  float* dq = reinterpret_cast<float*>(ws + p.dq);
-  float* pw = reinterpret_cast<float*>(ws + p.dw);
-  float* pk = reinterpret_cast<float*>(ws + p.dk);
-  if (dx || dwq)
-    router_dq_kernel<T><<<(int)std::min<int64_t>((M + 7) / 8, sms * 8), 256, 0, st>>>(ds, k16, q16, rnorm, M, NB, dq);
-  if (dk16) {
-    const int n = NB * kIdx;
-    router_dk_kernel<<<dim3((n + 255) / 256, p.parts), 256, 0, st>>>(ds, q16, M, NB, p.chunk, pk);
-    if (grad_dtype == FP_DTYPE_BF16)
-      sum_partials_kernel<<<(n + 255) / 256, 256, 0, st>>>(pk, p.parts, n, (__nv_bfloat16*)dk16);
+               int grad_dtype, char* ws, cudaStream_t st) {
+  const BwdPlan p = bwd_plan(sizeof(T) == 2 ? FP_DTYPE_BF16 : FP_DTYPE_F32, M, D, NB);
+  void* dq = dx || dwq ? ws + p.dq : nullptr;
+  float* pw = dwq ? reinterpret_cast<float*>(ws + p.dw) : nullptr;
+  float* pk = dk16 ? reinterpret_cast<float*>(ws + p.dk) : nullptr;
+  int rc;
+  if (NB <= 128) rc = launch_dq<T, 1>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  else if (NB <= 256) rc = launch_dq<T, 2>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  else if (NB <= 512) rc = launch_dq<T, 4>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  else rc = launch_dq<T, 8>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  if (rc) return rc;
+  if (dq) {
+    const dim3 grid(p.col_ctas, p.parts);
+    cudaError_t e;
+    if constexpr (sizeof(T) == 2)
+      e = launch_pdl(codes ? router_x_kernel<true> : router_x_kernel<false>, grid, kXWarps * 32, 0, st, x, codes, scales,
+                     (const uint4*)dq, wq, M, D, p.wide, p.per_cta, dx, pw);
     else
-      sum_partials_kernel<<<(n + 255) / 256, 256, 0, st>>>(pk, p.parts, n, (float*)dk16);
+      e = launch_pdl(codes ? router_x_f32_kernel<true> : router_x_f32_kernel<false>, grid, kFThreads, 0, st, x, codes,
+                     scales, (const float*)dq, wq, M, D, p.wide, p.per_cta, dx, pw);
+    if (e != cudaSuccess) return FP_ERR_CUDA;
   }
-  if (dwq) {
-    const int64_t n = (int64_t)kIdx * D;
-    router_dw_kernel<T><<<dim3((D + 255) / 256, p.parts), 256, 0, st>>>(x, codes, scales, dq, M, D, p.chunk, pw);
+  if (dwq || dk16) {
+    const int64_t n1 = dwq ? (int64_t)kIdx * D : 0, n2 = dk16 ? (int64_t)kIdx * NB : 0;
+    const unsigned grid = (unsigned)((n1 + 31) / 32 + (n2 + 31) / 32);
+    cudaError_t e;
     if (grad_dtype == FP_DTYPE_BF16)
-      sum_partials_kernel<<<(int)((n + 255) / 256), 256, 0, st>>>(pw, p.parts, n, (__nv_bfloat16*)dwq);
+      e = launch_pdl(sum_partials_kernel<__nv_bfloat16>, grid, 256, 0, st, pw, p.parts, n1, (__nv_bfloat16*)dwq, pk,
+                     p.dq_ctas, n2, (__nv_bfloat16*)dk16);
     else
-      sum_partials_kernel<<<(int)((n + 255) / 256), 256, 0, st>>>(pw, p.parts, n, (float*)dwq);
+      e = launch_pdl(sum_partials_kernel<float>, grid, 256, 0, st, pw, p.parts, n1, (float*)dwq, pk, p.dq_ctas, n2,
+                     (float*)dk16);
+    if (e != cudaSuccess) return FP_ERR_CUDA;
   }
-  if (dx)
-    router_dx_kernel<T><<<(int)std::min<int64_t>((M * D + 255) / 256, sms * 16), 256, 0, st>>>(dq, wq, M, D, dx);
   return launched();
 }
 
@@ -380,8 +786,8 @@ int fp_router_scores_train(const void* x, const void* q_proj, const void* block_
   return codes ? fp_mxfp8_quantize(x, dtype, M * D, codes, scales, stream) : FP_OK;
 }
 
-size_t fp_router_scores_bwd_workspace_size(int64_t M, int D, int NB) {
-  return M > 0 && D > 0 && NB > 0 ? bwd_plan(M, D, NB).total : 256;
+size_t fp_router_scores_bwd_workspace_size(int dtype, int64_t M, int D, int NB) {
+  return M > 0 && D > 0 && NB > 0 ? bwd_plan(dtype, M, D, NB).total : 256;
 }
 
 int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes, const void* scales,
@@ -397,7 +803,7 @@ int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes,
   if ((codes == nullptr) != (scales == nullptr)) return FP_ERR_INVALID_ARG;
   if (!al16(x) || !al16(codes) || !al16(q_proj) || !al16(dx) || !al16(dscores) || !al16(q16) || !al16(workspace))
     return FP_ERR_INVALID_ARG;
-  if (workspace_bytes < bwd_plan(M, D, NB).total) return FP_ERR_WORKSPACE;
+  if (workspace_bytes < bwd_plan(dtype, M, D, NB).total) return FP_ERR_WORKSPACE;
   int sms;
   if (const int rc = device_info(sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
@@ -405,10 +811,10 @@ int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes,
   if (dtype == FP_DTYPE_BF16)
     return router_bwd(dscores, (const __nv_bfloat16*)x, (const uint8_t*)codes, (const uint8_t*)scales,
                       (const __nv_bfloat16*)q_proj, (const __nv_bfloat16*)block_keys, q16, rnorm, M, D, NB,
-                      (__nv_bfloat16*)dx, dq_proj, dblock_keys, grad_dtype, ws, sms, st);
+                      (__nv_bfloat16*)dx, dq_proj, dblock_keys, grad_dtype, ws, st);
   return router_bwd(dscores, (const float*)x, (const uint8_t*)codes, (const uint8_t*)scales, (const float*)q_proj,
                     (const float*)block_keys, q16, rnorm, M, D, NB, (float*)dx, dq_proj, dblock_keys, grad_dtype, ws,
-                    sms, st);
+                    st);
 }
 
 size_t fp_balance_workspace_size(int64_t M, int NB) {

@@ -264,7 +264,7 @@ def router_scores_bwd(dscores: torch.Tensor, x2d: Optional[torch.Tensor], buf: O
         dk = torch.empty(NB, 16, dtype=grad_dtype, device=dev) if want[2] else None
         if M == 0:
             return dx, dw.zero_() if dw is not None else None, dk.zero_() if dk is not None else None
-        nbytes = lib.fp_router_scores_bwd_workspace_size(M, D, NB)
+        nbytes = lib.fp_router_scores_bwd_workspace_size(dt, M, D, NB)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         codes, scales = _mx_ptrs(buf, M * D) if buf is not None else (None, None)
         check(lib.fp_router_scores_bwd(ptr(dscores), ptr(x2d), codes, scales, ptr(q_proj), ptr(block_keys), ptr(q16),

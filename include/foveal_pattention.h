@@ -479,7 +479,7 @@ FP_API int fp_router_scores_train(const void* x, const void* q_proj, const void*
  * computed).  x may be NULL when codes and scales are given (its MXFP8 copy is read then, also when x is
  * given) or dq_proj is not wanted.  The sums over tokens have a fixed order.
  */
-FP_API size_t fp_router_scores_bwd_workspace_size(int64_t M, int D, int NB);
+FP_API size_t fp_router_scores_bwd_workspace_size(int dtype, int64_t M, int D, int NB);
 FP_API int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes, const void* scales,
                                 const void* q_proj, const void* block_keys, const float* q16, const float* rnorm,
                                 int dtype, int64_t M, int D, int NB, void* dx, void* dq_proj, void* dblock_keys,

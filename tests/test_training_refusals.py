@@ -145,8 +145,8 @@ def test_c_router(lib):
     assert f(A, A, A, 5, 4, 64, 8, A, A, A, None, None, None) == UNSUPPORTED
     assert f(A, A, A, 1, 4, 64, 8, A, A, A, A, None, None) == INVALID
     assert f(A, A, A, 1, 4, 64, 8, A, A, A, ODD, A, None) == INVALID
-    n = w(4, 64, 8)
-    assert n > 0 and w(0, 0, 0) > 0
+    n = w(1, 4, 64, 8)
+    assert n > 0 and w(1, 0, 0, 0) > 0
 
     def go(ds=A, x=A, c=None, s=None, wq=A, k=A, q=A, r=A, dt=1, M=4, D=64, NB=8, dx=A, dw=A, dk=A, gd=0, ws=A, nb=n):
         return b(ds, x, c, s, wq, k, q, r, dt, M, D, NB, dx, dw, dk, gd, ws, nb, None)
