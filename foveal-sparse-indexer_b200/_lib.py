@@ -176,6 +176,12 @@ def on_device(device: torch.device):
     return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream of ``device`` as an address (:func:`stream_handle` without its Stream object, whose
+    construction takes longer than a launch)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous()
 

@@ -28,11 +28,6 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
 
 // ------------------------------------------------------------------ gradient of the scores
 // Three launches.  (1) One pass over dS: dq of every token and partial sums of dK.  (2) One pass over x: dx and
@@ -575,181 +570,417 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
 }
 
 // ------------------------------------------------------------------ balance loss
-constexpr int kBalWarps = 8;
-constexpr int kBalMaxCtas = 296;
+// A warp takes kR rows at a time, each row's scores in its registers (kE to a lane), with all of the rows'
+// loads issued before the first use.  What bounds the passes is the instructions of a row (about 230 forward
+// with its list, 240 backward at 448 blocks) and, below some 10^4 rows, latency and the number of partial sums
+// that the join has to read: CTAs in clusters of 8 add their column sums through distributed shared memory.
+// 256 CTAs, not two to each of 148 SMs: 37 clusters of 8 are not resident at once, and the last ones ran alone
+// (65521 x 448: forward 70 us with 296 CTAs, 51 us with 256; clusters of 4: 76 us with 288, 55 us with 256).
+constexpr int kBalWarps = 16;
+constexpr int kBalCluster = 8;
+constexpr int kBalMaxCtas = 256;
+constexpr int kGradWarps = 8;
 
-// One row's remote scores in a warp's registers, divided by T; returns whether the row is counted, and turns
-// the scores into probabilities.  A row whose remote scores are all -inf has no distribution and is not
-// counted; a NaN makes the whole row NaN.
-template <int E>
-__device__ __forceinline__ bool balance_row(const float* __restrict__ row, int NB, int base, float temperature,
-                                            int lane, float (&p)[E]) {
-  float top = -INFINITY;
-  bool nan = false;
+template <int kE>
+constexpr int kRowsOf = kE <= 4 ? 4 : kE == 8 ? 2 : 1;
+
+// Column of a lane's i-th score: quads of columns where rows are 16-byte aligned (kVec), else single ones.
+template <bool kVec>
+__device__ __forceinline__ int bal_col(int lane, int i) {
+  return kVec ? 4 * lane + 128 * (i >> 2) + (i & 3) : lane + 32 * i;
+}
+template <int kE, bool kVec>
+__device__ __forceinline__ void bal_load(const float* __restrict__ row, int NB, int lane, float (&z)[kE]) {
+  if constexpr (kVec) {
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int b = lane + 32 * i;
-    float z = -INFINITY;
-    if (b >= base && b < NB) {
-      z = row[b];
-      if (temperature != 1.0f) z = __fdiv_rn(z, temperature);
+    for (int i = 0; i < kE / 4; ++i) {
+      const int b = 4 * lane + 128 * i;
+      const float4 v = b < NB ? __ldg(reinterpret_cast<const float4*>(row + b))
+                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      z[4 * i] = v.x; z[4 * i + 1] = v.y; z[4 * i + 2] = v.z; z[4 * i + 3] = v.w;
     }
-    nan |= z != z;
-    top = fmaxf(top, z);
-    p[i] = z;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) z[i] = lane + 32 * i < NB ? __ldg(row + lane + 32 * i) : -INFINITY;
   }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Largest value over the warp; a NaN loses.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Scores (-inf past the row's end) to exp((z - max) / T) over the remote blocks, 0 for the base blocks; `sum` is
+// the lane's part of their sum.  Returns whether the row is counted: a row whose remote scores are all -inf
+// has no distribution and is not; a NaN makes the whole row NaN.  c = log2(e) / T.  The passes are issue bound
+// at 448 blocks (24 instructions a score before, about 7 now), hence one fused multiply-add and the hardware
+// exponential per score: 2^-22 of p, next to the rounding of z c (|z| c 2^-24).
+template <int kE, bool kVec>
+__device__ __forceinline__ bool bal_exp(float (&z)[kE], int base, float c, int lane, float& sum) {
+  constexpr int kHead = kVec ? 4 : 4 < kE ? 4 : kE;  // elements in a lane's first 128 columns
+#pragma unroll
+  for (int i = 0; i < kHead; ++i)
+    if (bal_col<kVec>(lane, i) < base) z[i] = -INFINITY;
+  if (base > 128) {
+#pragma unroll
+    for (int i = kHead; i < kE; ++i)
+      if (bal_col<kVec>(lane, i) < base) z[i] = -INFINITY;
+  }
+  float top = z[0];
+#pragma unroll
+  for (int i = 1; i < kE; ++i) top = fmaxf(top, z[i]);
   top = warp_max(top);
-  if (top == -INFINITY && !__any_sync(0xffffffffu, nan)) return false;
-  float sum = 0.f;
+  const float d = -top * c;
+  sum = 0.f;
+  if (fabsf(d) <= 1e38f) {
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int b = lane + 32 * i;
-    p[i] = b >= base && b < NB ? expf(p[i] - top) : 0.f;
-    sum += p[i];
+    for (int i = 0; i < kE; ++i) z[i] = exp2_fast(fmaf(z[i], c, d));
+  } else {  // nothing above -inf, an infinity, or scores of the type's lowest value (a mask) only
+    if (top == -INFINITY) {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < kE; ++i) nan |= z[i] != z[i];
+      if (!__any_sync(0xffffffffu, nan)) return false;
+      top = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const float e = z[i] - top;  // equal scores: exactly 0
+      z[i] = e == 0.f ? 1.f : exp2_fast(e * c);
+    }
   }
-  const float inv = __fdiv_rn(1.0f, warp_sum(sum));
 #pragma unroll
-  for (int i = 0; i < E; ++i) p[i] *= inv;
+  for (int i = 0; i < kE; ++i) sum += z[i];
   return true;
 }
 
-// Per CTA: column sums of p over its rows, the number of counted rows, and the blocks' slot counts.
+// Per cluster: column sums of p over its rows, the number of counted rows, and the blocks' slot counts.
 // scores may be NULL (counts only); idx may be NULL (counts given).
-template <int E>
-__global__ void __launch_bounds__(kBalWarps * 32)
+//
+// Counting: shared-memory atomics and plain byte flags take about the same time here, but flags need a third of
+// the instructions.  A row's list sets one byte per block in the warp's own shared memory; each lane adds the
+// four columns of its words to byte counters in registers (spilled to the CTA's counts every 255 rows) and
+// clears them.  A list that names a block twice is noticed by its sum and counted with atomics.
+template <int kE, bool kVec>
+__global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalWarps * 32, kE <= 16 ? 2 : 1)
 balance_partial_kernel(const float* __restrict__ scores, int64_t M, int NB, int base, float temperature,
                        const uint8_t* __restrict__ valid, const int32_t* __restrict__ idx,
                        const int32_t* __restrict__ cnt, int capacity, float* __restrict__ psum,
                        int32_t* __restrict__ rows, int32_t* __restrict__ hist) {
-  extern __shared__ float sm[];  // [kBalWarps][NB] column sums, then [NB] slot counts
-  int* sh = reinterpret_cast<int*>(sm + kBalWarps * NB);
+  constexpr int kR = kRowsOf<kE>;
+  constexpr int kW = kE < 4 ? 1 : kE / 4;    // words of four byte counters in a lane
+  constexpr int kL = kE <= 2 ? 2 : 4;        // list entries of a row that a lane loads ahead
+  // [NB] column sums, [NB] slot counts, [kBalWarps][NB] the warps' sums, of which each warp uses its first NB
+  // bytes as its flags before the sums are written
+  extern __shared__ float sm[];
+  int* sh = reinterpret_cast<int*>(sm + NB);
+  float* sw = sm + 2 * NB;
   __shared__ int s_rows;
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < NB; i += blockDim.x) sh[i] = 0;
   if (threadIdx.x == 0) s_rows = 0;
+  uint8_t* flags = reinterpret_cast<uint8_t*>(sw + warp * NB);
+  uint32_t* flag4 = reinterpret_cast<uint32_t*>(flags);
+#pragma unroll
+  for (int i = 0; i < kW; ++i)
+    if (4 * lane + 128 * i < NB) flag4[lane + 32 * i] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float acc[E];
+  float acc[kE];
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc[i] = 0.f;
-  int counted = 0;
-  for (int64_t t = (int64_t)blockIdx.x * kBalWarps + warp; t < M; t += (int64_t)gridDim.x * kBalWarps) {
-    if (valid && !valid[t]) continue;
-    if (idx) {
-      const int n = min(cnt[t], capacity);
-      for (int k = lane; k < n; k += 32) {
-        const int b = idx[t * capacity + k];
-        if (b >= 0 && b < NB) atomicAdd(&sh[b], 1);
+  for (int i = 0; i < kE; ++i) acc[i] = 0.f;
+  uint32_t slots[kW] = {};
+  int pending = 0, counted = 0;
+  const float c = fminf(__fdiv_rn(1.4426950408889634f, temperature), 3.4028234663852886e38f);
+  const int64_t step = (int64_t)gridDim.x * kBalWarps;
+  const bool lists = idx != nullptr;
+  for (int64_t t0 = (int64_t)blockIdx.x * kBalWarps + warp;; t0 += step * kR) {
+    const bool last = t0 >= M;
+    if (pending > 255 - kR || last) {  // byte counters to the CTA's counts
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        for (int k = 0; k < 4; ++k) {
+          const int n = (int)(slots[i] >> (8 * k) & 0xFF);
+          if (n) atomicAdd(&sh[4 * lane + 128 * i + k], n);
+        }
+        slots[i] = 0;
       }
+      pending = 0;
+      if (last) break;
     }
-    if (scores) {
-      float p[E];
-      if (balance_row<E>(scores + t * NB, NB, base, temperature, lane, p)) {
-        ++counted;
+    float z[kR][kE];
+    bool on[kR];
+    int n[kR], id[kR][kL];
 #pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] += p[i];
+    for (int r = 0; r < kR; ++r) {
+      const int64_t t = t0 + r * step;
+      on[r] = t < M;
+      if (scores && on[r]) bal_load<kE, kVec>(scores + t * NB, NB, lane, z[r]);
+      n[r] = 0;
+      if (lists && on[r]) {
+        n[r] = min(__ldg(cnt + t), capacity);
+        const int32_t* list = idx + t * capacity + lane;
+#pragma unroll
+        for (int k = 0; k < kL; ++k) id[r][k] = lane + 32 * k < capacity ? __ldg(list + 32 * k) : -1;
+      }
+      if (valid && on[r]) on[r] = __ldg(valid + t) != 0;
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+      if (!on[r]) continue;
+      if (n[r] > 0) {
+        const int32_t* list = idx + (t0 + r * step) * capacity;
+        int named = 0;
+#pragma unroll
+        for (int k = 0; k < kL; ++k)
+          if (lane + 32 * k < n[r] && (unsigned)id[r][k] < (unsigned)NB) {
+            flags[id[r][k]] = 1;
+            ++named;
+          }
+        for (int k = lane + 32 * kL; k < n[r]; k += 32) {
+          const int b = __ldg(list + k);
+          if ((unsigned)b < (unsigned)NB) {
+            flags[b] = 1;
+            ++named;
+          }
+        }
+        __syncwarp();
+        uint32_t f[kW];
+#pragma unroll
+        for (int i = 0; i < kW; ++i) {
+          f[i] = 0;
+          if (4 * lane + 128 * i < NB) {
+            f[i] = flag4[lane + 32 * i];
+            flag4[lane + 32 * i] = 0;
+            named -= __popc(f[i]);
+          }
+        }
+        __syncwarp();
+        if (__reduce_add_sync(0xffffffffu, named) == 0) {
+          ++pending;
+#pragma unroll
+          for (int i = 0; i < kW; ++i) slots[i] += f[i];
+        } else {
+          for (int k = lane; k < n[r]; k += 32) {
+            const int b = __ldg(list + k);
+            if ((unsigned)b < (unsigned)NB) atomicAdd(&sh[b], 1);
+          }
+        }
+      }
+      float sum;
+      if (scores && bal_exp<kE, kVec>(z[r], base, c, lane, sum)) {
+        ++counted;
+        const float inv = rcp_fast(warp_sum(sum));
+#pragma unroll
+        for (int i = 0; i < kE; ++i) acc[i] = fmaf(z[r][i], inv, acc[i]);
       }
     }
   }
+  __syncwarp();  // the flags' place now takes the sums
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (lane + 32 * i < NB) sm[warp * NB + lane + 32 * i] = acc[i];
+  for (int i = 0; i < kE; ++i)
+    if (bal_col<kVec>(lane, i) < NB) sw[warp * NB + bal_col<kVec>(lane, i)] = acc[i];
   if (lane == 0) atomicAdd(&s_rows, counted);
   __syncthreads();
   for (int b = threadIdx.x; b < NB; b += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kBalWarps; ++w) s += sm[w * NB + b];
-    psum[(int64_t)blockIdx.x * NB + b] = s;
-    hist[(int64_t)blockIdx.x * NB + b] = sh[b];
+    for (int w = 0; w < kBalWarps; ++w) s += sw[w * NB + b];
+    sm[b] = s;
+  }
+  cluster_sync();
+  const int rank = (int)cluster_ctarank(), part = blockIdx.x / kBalCluster;
+  for (int b = rank + kBalCluster * threadIdx.x; b < NB; b += kBalCluster * blockDim.x) {
+    float s = 0.f;
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < kBalCluster; ++k) {
+      s += ld_cluster_f32(sm + b, k);
+      c += __float_as_int(ld_cluster_f32(reinterpret_cast<const float*>(sh + b), k));
+    }
+    psum[(int64_t)part * NB + b] = s;
+    hist[(int64_t)part * NB + b] = c;
   }
   if (threadIdx.x == 0) rows[blockIdx.x] = s_rows;
+  cluster_sync();  // no CTA leaves while another reads its shared memory
 }
 
-// One CTA: joins the partials in their order, writes the counts, the loss and what the gradient needs:
-// state[b] = f_b - 1/R (0 when nothing was routed) and state[NB] = R / (T n).
+// One CTA of 1024 threads, `width` (a power of two >= NB) columns by 1024 / width groups of the partials: joins
+// them in their order, writes the counts, the loss and what the gradient needs: state[b] = f_b - 1/R (0 when
+// nothing was routed) and state[NB] = R / (T n).
 __global__ void __launch_bounds__(1024)
 balance_join_kernel(const float* __restrict__ psum, const int32_t* __restrict__ rows,
-                    const int32_t* __restrict__ hist, int parts, int NB, int base, float temperature,
+                    const int32_t* __restrict__ hist, int ctas, int NB, int width, int base, float temperature,
                     const int64_t* __restrict__ counts_in, int64_t* __restrict__ counts, float* __restrict__ loss,
                     float* __restrict__ state) {
-  __shared__ unsigned long long s_total;
-  __shared__ long long s_rows;
+  __shared__ double s_p[1024];
+  __shared__ long long s_c[1024];
   __shared__ double s_loss[32];
-  const int b = threadIdx.x, lane = b & 31, warp = b >> 5;
-  if (b == 0) {
-    s_total = 0;
-    long long r = 0;
-    for (int i = 0; i < parts; ++i) r += rows[i];
-    s_rows = r;
-  }
+  __shared__ long long s_tot[32];
+  __shared__ int s_rows;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = tid & (width - 1), grp = tid / width, groups = 1024 / width, parts = ctas / kBalCluster;
+  if (tid == 0) s_rows = 0;
+  griddep_wait();
   __syncthreads();
   int64_t c = 0;
   double ps = 0.0;
   if (b < NB) {
-    if (counts_in) c = counts_in[b];
-    for (int i = 0; i < parts; ++i) {
+#pragma unroll 8
+    for (int i = grp; i < parts; i += groups) {
       if (!counts_in) c += hist[(int64_t)i * NB + b];
       ps += (double)psum[(int64_t)i * NB + b];
     }
-    if (counts) counts[b] = c;
-    if (c) atomicAdd(&s_total, (unsigned long long)c);
   }
+  if (tid < ctas) atomicAdd(&s_rows, rows[tid]);
+  s_p[tid] = ps;
+  s_c[tid] = c;
   __syncthreads();
+  if (grp == 0) {
+    for (int k = 1; k < groups; ++k) {
+      ps += s_p[b + k * width];
+      c += s_c[b + k * width];
+    }
+    if (b < NB) {
+      if (counts_in) c = counts_in[b];
+      if (counts) counts[b] = c;
+    }
+  } else {
+    c = 0;
+  }
   if (!loss) return;
-  const int64_t total = (int64_t)s_total, n = s_rows;
-  const int R = NB - base;
-  const bool remote = b >= base && b < NB;
-  const double f = total > 0 && remote ? (double)c / (double)total : 0.0;
-  double part = remote ? f * ps : 0.0;
+  int64_t tot = c;
+  for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+  if (lane == 0) s_tot[warp] = tot;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < 32; ++w) total += s_tot[w];
+  const int R = NB - base, n = s_rows;
+  const bool remote = grp == 0 && b >= base && b < NB;
+  double part = remote && total > 0 ? (double)c / (double)total * ps : 0.0;
   for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
   if (lane == 0) s_loss[warp] = part;
   __syncthreads();
-  if (b == 0) {
+  if (tid == 0) {
     double s = 0.0;
     for (int w = 0; w < 32; ++w) s += s_loss[w];
-    *loss = n > 0 ? (float)(s * R / (double)n) : (float)s;
+    *loss = n > 0 ? (float)(s * R / (double)n) : 0.f;
     state[NB] = n > 0 ? (float)((double)R / ((double)temperature * (double)n)) : 0.f;
   }
-  if (b < NB)
+  if (grp == 0 && b < NB)
     state[b] = total > 0 && remote ? (float)((double)(c * R - total) / ((double)total * R)) : 0.f;
 }
 
-template <int E>
-__global__ void __launch_bounds__(kBalWarps * 32)
+template <int kE, bool kVec>
+__global__ void __launch_bounds__(kGradWarps * 32)
 balance_grad_kernel(const float* __restrict__ scores, int64_t M, int NB, int base, float temperature,
                     const uint8_t* __restrict__ valid, const float* __restrict__ state,
                     const float* __restrict__ dloss, float* __restrict__ ds) {
+  constexpr int kR = kRowsOf<kE>;
+  constexpr int kHead = kVec ? 4 : 4 < kE ? 4 : kE;
   const int lane = threadIdx.x & 31;
   const float scale = state[NB] * *dloss;
-  float f[E];
+  const float c = fminf(__fdiv_rn(1.4426950408889634f, temperature), 3.4028234663852886e38f);
+  float f[kE];
 #pragma unroll
-  for (int i = 0; i < E; ++i) f[i] = lane + 32 * i < NB ? state[lane + 32 * i] : 0.f;
-  for (int64_t t = (int64_t)blockIdx.x * kBalWarps + (threadIdx.x >> 5); t < M; t += (int64_t)gridDim.x * kBalWarps) {
-    float p[E];
-    const bool counted = (!valid || valid[t]) && balance_row<E>(scores + t * NB, NB, base, temperature, lane, p);
-    float inner = 0.f;
-    if (counted) {
+  for (int i = 0; i < kE; ++i) f[i] = bal_col<kVec>(lane, i) < NB ? state[bal_col<kVec>(lane, i)] : 0.f;
+  const int64_t step = (int64_t)gridDim.x * kGradWarps;
+  for (int64_t t0 = (int64_t)blockIdx.x * kGradWarps + (threadIdx.x >> 5); t0 < M; t0 += step * kR) {
+    float p[kR][kE];
+    bool on[kR];
 #pragma unroll
-      for (int i = 0; i < E; ++i) inner = fmaf(p[i], f[i], inner);
-      inner = warp_sum(inner);
+    for (int r = 0; r < kR; ++r) {
+      const int64_t t = t0 + r * step;
+      on[r] = t < M;
+      if (on[r]) bal_load<kE, kVec>(scores + t * NB, NB, lane, p[r]);
+      if (on[r] && valid) on[r] = __ldg(valid + t) != 0;
     }
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int b = lane + 32 * i;
-      if (b < NB) ds[t * NB + b] = counted && b >= base ? p[i] * (f[i] - inner) * scale : 0.f;
+    for (int r = 0; r < kR; ++r) {
+      const int64_t t = t0 + r * step;
+      if (t >= M) break;
+      float sum;
+      const bool counted = on[r] && bal_exp<kE, kVec>(p[r], base, c, lane, sum);
+      if (counted) {
+        float inner = 0.f;
+#pragma unroll
+        for (int i = 0; i < kE; ++i) inner = fmaf(p[r][i], f[i], inner);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          inner += __shfl_xor_sync(0xffffffffu, inner, o);
+        }
+        const float inv = rcp_fast(sum), k = scale * inv, m = -inner * inv * k;
+#pragma unroll
+        for (int i = 0; i < kE; ++i) p[r][i] *= fmaf(f[i], k, m);
+#pragma unroll
+        for (int i = 0; i < kHead; ++i)
+          if (bal_col<kVec>(lane, i) < base) p[r][i] = 0.f;  // also in a NaN row
+        if (base > 128) {
+#pragma unroll
+          for (int i = kHead; i < kE; ++i)
+            if (bal_col<kVec>(lane, i) < base) p[r][i] = 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kE; ++i) p[r][i] = 0.f;
+      }
+      float* o = ds + t * NB;
+      if constexpr (kVec) {
+#pragma unroll
+        for (int i = 0; i < kE / 4; ++i)
+          if (4 * lane + 128 * i < NB)
+            *reinterpret_cast<float4*>(o + 4 * lane + 128 * i) =
+                make_float4(p[r][4 * i], p[r][4 * i + 1], p[r][4 * i + 2], p[r][4 * i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kE; ++i)
+          if (lane + 32 * i < NB) o[lane + 32 * i] = p[r][i];
+      }
     }
   }
 }
 
-int balance_ctas(int64_t M) { return (int)std::max<int64_t>(1, std::min<int64_t>((M + kBalWarps - 1) / kBalWarps, kBalMaxCtas)); }
+int balance_ctas(int64_t M) {
+  const int64_t want = (M + kBalWarps * 2 - 1) / (kBalWarps * 2);  // two rows to a warp
+  const int64_t up = (want + kBalCluster - 1) / kBalCluster * kBalCluster;
+  return (int)std::max<int64_t>(kBalCluster, std::min<int64_t>(up, kBalMaxCtas));
+}
 
-template <int E>
-void balance_fwd_go(const float* scores, int64_t M, int NB, int base, float temperature, const uint8_t* valid,
-                    const int32_t* idx, const int32_t* cnt, int capacity, float* psum, int32_t* rows, int32_t* hist,
-                    cudaStream_t st) {
-  const size_t smem = (size_t)(kBalWarps + 1) * NB * 4;  // at most 36 KB
-  balance_partial_kernel<E><<<balance_ctas(M), kBalWarps * 32, smem, st>>>(
-      scores, M, NB, base, temperature, valid, idx, cnt, capacity, psum, rows, hist);
+template <int kE, bool kVec>
+int balance_fwd_go(const float* scores, int64_t M, int NB, int base, float temperature, const uint8_t* valid,
+                   const int32_t* idx, const int32_t* cnt, int capacity, float* psum, int32_t* rows, int32_t* hist,
+                   cudaStream_t st) {
+  const auto kern = balance_partial_kernel<kE, kVec>;
+  const size_t smem = (size_t)(kBalWarps + 2) * NB * 4;  // at most 72 KB
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return FP_ERR_CUDA;
+  kern<<<balance_ctas(M), kBalWarps * 32, smem, st>>>(scores, M, NB, base, temperature, valid, idx, cnt, capacity,
+                                                      psum, rows, hist);
+  return launched();
+}
+
+template <int kE, bool kVec>
+int balance_bwd_go(const float* scores, int64_t M, int NB, int base, float temperature, const uint8_t* valid,
+                   const float* state, const float* dloss, float* ds, int sms, cudaStream_t st) {
+  const int64_t rows = (int64_t)kGradWarps * kRowsOf<kE>;
+  const int grid = (int)std::min<int64_t>((M + rows - 1) / rows, (int64_t)sms * 8);
+  balance_grad_kernel<kE, kVec><<<grid, kGradWarps * 32, 0, st>>>(scores, M, NB, base, temperature, valid, state, dloss,
+                                                                 ds);
+  return launched();
 }
 
 }  // namespace
@@ -757,14 +988,25 @@ void balance_fwd_go(const float* scores, int64_t M, int NB, int base, float temp
 
 using namespace fp;
 
-#define FP_BY_WIDTH(NB, CALL)                 \
-  do {                                        \
-    if ((NB) <= 32) { constexpr int E = 1; CALL; }        \
-    else if ((NB) <= 64) { constexpr int E = 2; CALL; }   \
-    else if ((NB) <= 128) { constexpr int E = 4; CALL; }  \
-    else if ((NB) <= 256) { constexpr int E = 8; CALL; }  \
-    else if ((NB) <= 512) { constexpr int E = 16; CALL; } \
-    else { constexpr int E = 32; CALL; }      \
+// CALL with kE scores to a lane and kVec for the row width NB; rows are read in quads where they are 16-byte
+// aligned and wide enough to fill half a warp's.
+#define FP_BY_WIDTH(NB, ALIGNED, CALL)                                              \
+  do {                                                                              \
+    if ((ALIGNED) && (NB) % 4 == 0 && (NB) > 64) {                                  \
+      constexpr bool kVec = true;                                                   \
+      if ((NB) <= 128) { constexpr int kE = 4; CALL; }                              \
+      else if ((NB) <= 256) { constexpr int kE = 8; CALL; }                         \
+      else if ((NB) <= 512) { constexpr int kE = 16; CALL; }                        \
+      else { constexpr int kE = 32; CALL; }                                         \
+    } else {                                                                        \
+      constexpr bool kVec = false;                                                  \
+      if ((NB) <= 32) { constexpr int kE = 1; CALL; }                               \
+      else if ((NB) <= 64) { constexpr int kE = 2; CALL; }                          \
+      else if ((NB) <= 128) { constexpr int kE = 4; CALL; }                         \
+      else if ((NB) <= 256) { constexpr int kE = 8; CALL; }                         \
+      else if ((NB) <= 512) { constexpr int kE = 16; CALL; }                        \
+      else { constexpr int kE = 32; CALL; }                                         \
+    }                                                                               \
   } while (0)
 
 extern "C" {
@@ -818,7 +1060,7 @@ int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes,
 }
 
 size_t fp_balance_workspace_size(int64_t M, int NB) {
-  return M >= 0 && NB > 0 ? (size_t)balance_ctas(M) * (8 * (size_t)NB + 4) + 256 : 256;
+  return M >= 0 && NB > 0 ? (size_t)balance_ctas(M) * ((size_t)NB + 4) + 256 : 256;
 }
 
 int fp_balance_loss_fwd(const float* scores, int64_t M, int NB, int base_blocks, float temperature,
@@ -837,15 +1079,21 @@ int fp_balance_loss_fwd(const float* scores, int64_t M, int NB, int base_blocks,
   int sms;
   if (const int rc = device_info(sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  const int parts = balance_ctas(M);
+  const int ctas = balance_ctas(M), parts = ctas / kBalCluster;
   float* psum = (float*)workspace;
   int32_t* hist = (int32_t*)(psum + (size_t)parts * NB);
   int32_t* rows = hist + (size_t)parts * NB;
   const int32_t* idx = counts_in ? nullptr : remote_indices;
-  FP_BY_WIDTH(NB, balance_fwd_go<E>(loss ? scores : nullptr, M, NB, base_blocks, temperature, valid, idx,
-                                    remote_counts, capacity, psum, rows, hist, st));
-  balance_join_kernel<<<1, 1024, 0, st>>>(psum, rows, hist, parts, NB, base_blocks, temperature, counts_in, counts, loss,
-                                          state);
+  const float* s = loss ? scores : nullptr;
+  int rc = FP_OK;
+  FP_BY_WIDTH(NB, al16(scores), (rc = balance_fwd_go<kE, kVec>(s, M, NB, base_blocks, temperature, valid, idx, remote_counts,
+                                                              capacity, psum, rows, hist, st)));
+  if (rc) return rc;
+  int width = 32;
+  while (width < NB) width *= 2;
+  if (launch_pdl(balance_join_kernel, dim3(1), dim3(1024), 0, st, psum, rows, hist, ctas, NB, width, base_blocks,
+                 temperature, counts_in, counts, loss, state) != cudaSuccess)
+    return FP_ERR_CUDA;
   return launched();
 }
 
@@ -858,10 +1106,10 @@ int fp_balance_loss_bwd(const float* scores, int64_t M, int NB, int base_blocks,
   int sms;
   if (const int rc = device_info(sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  const int grid = (int)std::min<int64_t>((M + kBalWarps - 1) / kBalWarps, (int64_t)sms * 8);
-  FP_BY_WIDTH(NB, (balance_grad_kernel<E><<<grid, kBalWarps * 32, 0, st>>>(scores, M, NB, base_blocks, temperature,
-                                                                          valid, state, dloss, dscores)));
-  return launched();
+  int rc = FP_OK;
+  FP_BY_WIDTH(NB, al16(scores) && al16(dscores), (rc = balance_bwd_go<kE, kVec>(scores, M, NB, base_blocks, temperature, valid,
+                                                                               state, dloss, dscores, sms, st)));
+  return rc;
 }
 
 }  // extern "C"

@@ -74,7 +74,7 @@ class _PooledTrain(torch.autograd.Function):
         packed = module._packed()
         keep = module.checkpoint is not None
         if keep:
-            scores, q16, rnorm, buf = kernels.router_scores_train(x2d, wq, k16, keep_mxfp8=True)
+            scores, saved, buf = kernels.router_scores_train(x2d, wq, k16, keep_mxfp8=True)
         else:
             scores, _ = kernels.router_scores(x2d, wq, k16)
         active, _ = kernels.pooled_route(None, wq, k16, base_blocks=module.base_blocks,
@@ -85,7 +85,7 @@ class _PooledTrain(torch.autograd.Function):
         y = kernels.pooled_forward(x2d, k_gate, k_up, v, packed, active, ctx16=c16, out_proj=wout)
         ctx.x_shape, ctx.x_dtype = x2d.shape, x2d.dtype
         ctx.save_for_backward(buf if keep else x2d, k_gate, k_up, v, wq, k16, wout, scores, active,
-                              *((q16, rnorm) if keep else ()))
+                              *((saved,) if keep else ()))
         ctx.temperature = module.temperature
         ctx.block_size = module.block_size
         ctx.mark_non_differentiable(scores, active)

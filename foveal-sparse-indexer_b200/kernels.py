@@ -153,14 +153,18 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
 def mxfp8_nbytes(n: int) -> int:
     """Bytes of an n-element MXFP8 copy: codes, padded to 16 bytes, then one scale byte per 32 elements."""
     return (n + 15) // 16 * 16 + (n + 31) // 32
 
 
-def _mx_ptrs(buf: torch.Tensor, n: int, at: int = 0):
+def _mx_addrs(buf: torch.Tensor, n: int, at: int = 0) -> Tuple[int, int]:
     p = buf.data_ptr() + at
-    return ctypes.c_void_p(p), ctypes.c_void_p(p + (n + 15) // 16 * 16)
+    return p, p + (n + 15) // 16 * 16
 
 
 def mxfp8_quantize(x: torch.Tensor) -> torch.Tensor:
@@ -171,7 +175,8 @@ def mxfp8_quantize(x: torch.Tensor) -> torch.Tensor:
     n = x.numel()
     with _lib.on_device(dev):
         buf = torch.empty(mxfp8_nbytes(n), dtype=torch.uint8, device=dev)
-        check(_lib.load().fp_mxfp8_quantize(ptr(x), dt, n, *_mx_ptrs(buf, n), stream_handle(dev)), "fp_mxfp8_quantize")
+        check(_lib.load().fp_mxfp8_quantize(x.data_ptr(), dt, n, *_mx_addrs(buf, n), _lib.raw_stream(dev)),
+              "fp_mxfp8_quantize")
     return buf
 
 
@@ -184,7 +189,7 @@ def mxfp8_dequantize(buf: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tens
         n = y.numel()
         if buf.dtype != torch.uint8 or buf.numel() != mxfp8_nbytes(n):
             raise ValueError(f"an MXFP8 copy of {n} elements is {mxfp8_nbytes(n)} uint8, got {buf.numel()} {buf.dtype}")
-        check(_lib.load().fp_mxfp8_dequantize(*_mx_ptrs(_dense(buf), n), dt, n, ptr(y), stream_handle(dev)),
+        check(_lib.load().fp_mxfp8_dequantize(*_mx_addrs(_dense(buf), n), dt, n, y.data_ptr(), _lib.raw_stream(dev)),
               "fp_mxfp8_dequantize")
     return y
 
@@ -199,10 +204,10 @@ def swiglu_fwd_mxfp8(g: torch.Tensor, u: torch.Tensor) -> Tuple[torch.Tensor, to
     n = g.numel()
     half = (mxfp8_nbytes(n) + 15) // 16 * 16
     with _lib.on_device(dev):
-        h = torch.empty_like(g)
+        h = torch.empty(g.shape, dtype=g.dtype, device=dev)
         buf = torch.empty(2 * half, dtype=torch.uint8, device=dev)
-        check(_lib.load().fp_swiglu_fwd_mxfp8(ptr(g), ptr(u), dt, n, ptr(h), *_mx_ptrs(buf, n), *_mx_ptrs(buf, n, half),
-                                              stream_handle(dev)), "fp_swiglu_fwd_mxfp8")
+        check(_lib.load().fp_swiglu_fwd_mxfp8(g.data_ptr(), u.data_ptr(), dt, n, h.data_ptr(), *_mx_addrs(buf, n),
+                                              *_mx_addrs(buf, n, half), _lib.raw_stream(dev)), "fp_swiglu_fwd_mxfp8")
     return h, buf
 
 
@@ -215,105 +220,115 @@ def swiglu_bwd_mxfp8(dout: torch.Tensor, buf: torch.Tensor, want_h: bool = False
     half = (mxfp8_nbytes(n) + 15) // 16 * 16
     if buf.dtype != torch.uint8 or buf.numel() != 2 * half:
         raise ValueError("the buffer is not that of swiglu_fwd_mxfp8 for as many elements")
+    buf = _dense(buf)
     with _lib.on_device(dev):
         dg, du = torch.empty_like(dout), torch.empty_like(dout)
         h = torch.empty_like(dout) if want_h else None
-        check(_lib.load().fp_swiglu_bwd_mxfp8(ptr(dout), *_mx_ptrs(buf, n), *_mx_ptrs(buf, n, half), dt, n, ptr(dg),
-                                              ptr(du), ptr(h), stream_handle(dev)), "fp_swiglu_bwd_mxfp8")
+        check(_lib.load().fp_swiglu_bwd_mxfp8(dout.data_ptr(), *_mx_addrs(buf, n), *_mx_addrs(buf, n, half), dt, n,
+                                              dg.data_ptr(), du.data_ptr(), _addr(h), _lib.raw_stream(dev)),
+              "fp_swiglu_bwd_mxfp8")
     return dg, du, h
 
 
-def router_scores_train(x2d: torch.Tensor, q_proj: torch.Tensor, block_keys: torch.Tensor, keep_mxfp8: bool = False):
-    """:func:`router_scores` for training (``fp_router_scores_train``): (scores [M, NB], q16 [M, 16],
-    rnorm [M], MXFP8 copy of x or None)."""
-    dev = require_cuda(x2d, q_proj, block_keys)
-    dt = dtype_code(x2d.dtype)
-    x2d, q_proj, block_keys = _dense(x2d), _dense(q_proj.to(x2d.dtype)), _dense(block_keys.to(x2d.dtype))
-    M, D = x2d.shape
-    NB = block_keys.shape[0]
+def router_scores_train(x: torch.Tensor, q_proj: torch.Tensor, block_keys: torch.Tensor, keep_mxfp8: bool = False):
+    """:func:`router_scores` for training (``fp_router_scores_train``), x [..., D]: (scores [..., NB], what
+    :func:`router_scores_bwd` needs of them, MXFP8 copy of x or None).  The second is one fp32 buffer: q16
+    [M, 16], then rnorm [M]."""
+    dev = require_cuda(x, q_proj, block_keys)
+    dt = dtype_code(x.dtype)
+    x, q_proj, block_keys = _dense(x), _dense(q_proj.to(x.dtype)), _dense(block_keys.to(x.dtype))
+    D, NB = x.shape[-1], block_keys.shape[0]
+    M = x.numel() // D
     with _lib.on_device(dev):
-        scores = torch.empty(M, NB, dtype=torch.float32, device=dev)
+        scores = torch.empty(x.shape[:-1] + (NB,), dtype=torch.float32, device=dev)
         saved = torch.empty(17 * M, dtype=torch.float32, device=dev)
-        q16, rnorm = saved[:16 * M].view(M, 16), saved[16 * M:]
         buf = torch.empty(mxfp8_nbytes(M * D), dtype=torch.uint8, device=dev) if keep_mxfp8 else None
-        codes, scales = _mx_ptrs(buf, M * D) if keep_mxfp8 and M > 0 else (None, None)
-        check(_lib.load().fp_router_scores_train(ptr(x2d), ptr(q_proj), ptr(block_keys), dt, M, D, NB, ptr(scores),
-                                                 ptr(q16), ptr(rnorm), codes, scales, stream_handle(dev)),
-              "fp_router_scores_train")
-    return scores, q16, rnorm, buf
+        codes, scales = _mx_addrs(buf, M * D) if keep_mxfp8 and M > 0 else (None, None)
+        q16 = saved.data_ptr()
+        check(_lib.load().fp_router_scores_train(x.data_ptr(), q_proj.data_ptr(), block_keys.data_ptr(), dt, M, D, NB,
+                                                 scores.data_ptr(), q16, q16 + 64 * M, codes, scales,
+                                                 _lib.raw_stream(dev)), "fp_router_scores_train")
+    return scores, saved, buf
 
 
-def router_scores_bwd(dscores: torch.Tensor, x2d: Optional[torch.Tensor], buf: Optional[torch.Tensor],
-                      q_proj: torch.Tensor, block_keys: torch.Tensor, q16: torch.Tensor, rnorm: torch.Tensor,
-                      dtype: torch.dtype, grad_dtype: torch.dtype = torch.float32,
-                      want: Tuple[bool, bool, bool] = (True, True, True)):
-    """Gradient of the router scores (``fp_router_scores_bwd``): (dx, dq_proj, dblock_keys), None where not
-    ``want``ed.  The tokens come from ``x2d`` or, where given, from their MXFP8 copy ``buf``; ``dtype`` is
-    theirs."""
-    dev = require_cuda(dscores, x2d, buf, q_proj, block_keys, q16, rnorm)
+def router_scores_bwd(dscores: torch.Tensor, x: Optional[torch.Tensor], buf: Optional[torch.Tensor],
+                      q_proj: torch.Tensor, block_keys: torch.Tensor, saved: torch.Tensor, dtype: torch.dtype,
+                      grad_dtype: torch.dtype = torch.float32, want: Tuple[bool, bool, bool] = (True, True, True)):
+    """Gradient of the router scores (``fp_router_scores_bwd``): (dx [..., D], dq_proj, dblock_keys), None where
+    not ``want``ed.  dscores is [..., NB] fp32; the tokens come from ``x`` or, where given, from their MXFP8
+    copy ``buf``; ``dtype`` is theirs."""
+    dev = require_cuda(dscores, x, buf, q_proj, block_keys, saved)
     dt = dtype_code(dtype)
     dscores = _dense(dscores.float())
     q_proj, block_keys = _dense(q_proj.to(dtype)), _dense(block_keys.to(dtype))
-    x2d = _dense(x2d) if x2d is not None else None
-    q16, rnorm = _dense(q16), _dense(rnorm)
-    (M, NB), D = dscores.shape, q_proj.shape[1]
+    x = _dense(x) if x is not None else None
+    NB, D = dscores.shape[-1], q_proj.shape[1]
+    M = dscores.numel() // NB
+    if saved.numel() != 17 * M or (x is not None and x.numel() != M * D) or \
+            (buf is not None and buf.numel() != mxfp8_nbytes(M * D)) or block_keys.shape != (NB, 16):
+        raise ValueError("the tensors are not those of router_scores_train for these shapes")
     lib = _lib.load()
     with _lib.on_device(dev):
-        dx = torch.empty(M, D, dtype=dtype, device=dev) if want[0] else None
+        dx = torch.empty(dscores.shape[:-1] + (D,), dtype=dtype, device=dev) if want[0] else None
         dw = torch.empty(16, D, dtype=grad_dtype, device=dev) if want[1] else None
         dk = torch.empty(NB, 16, dtype=grad_dtype, device=dev) if want[2] else None
         if M == 0:
             return dx, dw.zero_() if dw is not None else None, dk.zero_() if dk is not None else None
         nbytes = lib.fp_router_scores_bwd_workspace_size(dt, M, D, NB)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        codes, scales = _mx_ptrs(buf, M * D) if buf is not None else (None, None)
-        check(lib.fp_router_scores_bwd(ptr(dscores), ptr(x2d), codes, scales, ptr(q_proj), ptr(block_keys), ptr(q16),
-                                       ptr(rnorm), dt, M, D, NB, ptr(dx), ptr(dw), ptr(dk), dtype_code(grad_dtype),
-                                       ptr(ws), nbytes, stream_handle(dev)), "fp_router_scores_bwd")
+        codes, scales = _mx_addrs(buf, M * D) if buf is not None else (None, None)
+        q16 = saved.data_ptr()
+        check(lib.fp_router_scores_bwd(dscores.data_ptr(), _addr(x), codes, scales, q_proj.data_ptr(),
+                                       block_keys.data_ptr(), q16, q16 + 64 * M, dt, M, D, NB, _addr(dx), _addr(dw),
+                                       _addr(dk), dtype_code(grad_dtype), ws.data_ptr(), nbytes,
+                                       _lib.raw_stream(dev)), "fp_router_scores_bwd")
     return dx, dw, dk
 
 
 def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[torch.Tensor],
                      remote_counts: Optional[torch.Tensor], num_blocks: int, base_blocks: int, temperature: float,
                      valid: Optional[torch.Tensor], counts_in: Optional[torch.Tensor] = None):
-    """Counts of the routed blocks and, where ``scores`` [M, NB] fp32 are given, the balance loss
-    (``fp_balance_loss_fwd``): (loss 0-d fp32 or None, counts [NB] int64, state [NB + 1] fp32 or None)."""
+    """Counts of the routed blocks and, where ``scores`` [..., NB] fp32 are given, the balance loss
+    (``fp_balance_loss_fwd``): (loss 0-d fp32 or None, counts [NB] int64, state [NB + 1] fp32 or None).
+    remote_indices [..., capacity] and remote_counts [...] int32, valid [...] bool."""
     dev = require_cuda(scores, remote_indices, remote_counts, valid, counts_in)
     scores = _dense(scores) if scores is not None else None
     idx = _dense(remote_indices.to(torch.int32)) if remote_indices is not None else None
     cnt = _dense(remote_counts.to(torch.int32)) if remote_counts is not None else None
     valid = _dense(valid) if valid is not None else None
-    counts_in = _dense(counts_in.to(torch.int64)) if counts_in is not None else None
-    M = scores.shape[0] if scores is not None else cnt.shape[0]
-    cap = idx.shape[1] if idx is not None else 0
+    counts_in = _dense(counts_in) if counts_in is not None else None
+    M = scores.numel() // num_blocks if scores is not None else cnt.numel()
+    cap = idx.shape[-1] if idx is not None else 0
     if cap == 0:  # no list to read; an empty tensor has no address
         idx = cnt
     lib = _lib.load()
+    loss = state = None
     with _lib.on_device(dev):
         counts = torch.empty(num_blocks, dtype=torch.int64, device=dev)
-        out = torch.empty(num_blocks + 2, dtype=torch.float32, device=dev) if scores is not None else None
-        loss, state = (out[0], out[1:]) if out is not None else (None, None)
+        if scores is not None:
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            state = torch.empty(num_blocks + 1, dtype=torch.float32, device=dev)
         nbytes = lib.fp_balance_workspace_size(M, num_blocks)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(lib.fp_balance_loss_fwd(ptr(scores), M, num_blocks, int(base_blocks), float(temperature), ptr(valid),
-                                      ptr(idx), ptr(cnt), cap, ptr(counts_in), ptr(counts), ptr(loss), ptr(state),
-                                      ptr(ws), nbytes, stream_handle(dev)), "fp_balance_loss_fwd")
+        check(lib.fp_balance_loss_fwd(_addr(scores), M, num_blocks, base_blocks, temperature, _addr(valid), _addr(idx),
+                                      _addr(cnt), cap, _addr(counts_in), counts.data_ptr(), _addr(loss), _addr(state),
+                                      ws.data_ptr(), nbytes, _lib.raw_stream(dev)), "fp_balance_loss_fwd")
     return loss, counts, state
 
 
 def balance_loss_bwd(scores: torch.Tensor, base_blocks: int, temperature: float, valid: Optional[torch.Tensor],
                      state: torch.Tensor, dloss: torch.Tensor) -> torch.Tensor:
-    """dscores [M, NB] of :func:`balance_loss_fwd` (``fp_balance_loss_bwd``)."""
+    """dscores [..., NB] of :func:`balance_loss_fwd` (``fp_balance_loss_bwd``)."""
     dev = require_cuda(scores, valid, state, dloss)
     scores = _dense(scores)
     valid = _dense(valid) if valid is not None else None
     dloss = dloss.float()
-    M, NB = scores.shape
+    NB = scores.shape[-1]
     with _lib.on_device(dev):
         ds = torch.empty_like(scores)
-        check(_lib.load().fp_balance_loss_bwd(ptr(scores), M, NB, int(base_blocks), float(temperature), ptr(valid),
-                                              ptr(state), ptr(dloss), ptr(ds), stream_handle(dev)),
-              "fp_balance_loss_bwd")
+        check(_lib.load().fp_balance_loss_bwd(scores.data_ptr(), scores.numel() // NB, NB, base_blocks, temperature,
+                                              _addr(valid), state.data_ptr(), dloss.data_ptr(), ds.data_ptr(),
+                                              _lib.raw_stream(dev)), "fp_balance_loss_bwd")
     return ds
 
 

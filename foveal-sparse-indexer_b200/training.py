@@ -69,19 +69,19 @@ def checkpoint_mxfp8(x: Tensor) -> MXFP8Checkpoint:
 
 class _RouterScores(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x2d, q_proj, block_keys, keep):
-        scores, q16, rnorm, buf = kernels.router_scores_train(x2d, q_proj, block_keys, keep_mxfp8=keep)
-        ctx.keep, ctx.dtype = keep, x2d.dtype
-        ctx.save_for_backward(buf if keep else x2d, q_proj, block_keys, q16, rnorm)
+    def forward(ctx, x, q_proj, block_keys, keep):
+        scores, saved, buf = kernels.router_scores_train(x, q_proj, block_keys, keep_mxfp8=keep)
+        ctx.keep, ctx.dtype = keep, x.dtype
+        ctx.save_for_backward(buf if keep else x, q_proj, block_keys, saved)
         return scores
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dscores):
-        kept, q_proj, block_keys, q16, rnorm = ctx.saved_tensors
+        kept, q_proj, block_keys, saved = ctx.saved_tensors
         one = q_proj.dtype == block_keys.dtype
         dx, dw, dk = kernels.router_scores_bwd(dscores, None if ctx.keep else kept, kept if ctx.keep else None, q_proj,
-                                               block_keys, q16, rnorm, ctx.dtype,
+                                               block_keys, saved, ctx.dtype,
                                                grad_dtype=q_proj.dtype if one else torch.float32,
                                                want=ctx.needs_input_grad[:3])
         if not one:
@@ -107,27 +107,21 @@ def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: 
         raise ValueError(f"the router takes widths that are multiples of 8 and 1 to 1024 blocks, got D {D}, NB {NB}")
     require_cuda(x, q_proj, block_keys)
     grad = torch.is_grad_enabled() and (x.requires_grad or q_proj.requires_grad or block_keys.requires_grad)
-    s = _RouterScores.apply(x.reshape(-1, D), q_proj, block_keys, grad and checkpoint is not None)
-    return s.view(*x.shape[:-1], NB)
+    return _RouterScores.apply(x, q_proj, block_keys, grad and checkpoint is not None)
 
 
-def _routes(remote_indices: Tensor, remote_counts: Tensor) -> Tuple[Tensor, Tensor]:
+def _check_routes(remote_indices: Tensor, remote_counts: Tensor) -> None:
     for t in (remote_indices, remote_counts):
         if t.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"remote_indices and remote_counts are int32 or int64, got {t.dtype}")
     if remote_indices.dim() < 1 or remote_indices.shape[:-1] != remote_counts.shape:
         raise ValueError(f"shapes: remote_indices [..., capacity], remote_counts [...]; got "
                          f"{tuple(remote_indices.shape)} and {tuple(remote_counts.shape)}")
-    M = remote_counts.numel()
-    return remote_indices.reshape(M, remote_indices.shape[-1]), remote_counts.reshape(M)
 
 
-def _valid(valid: Optional[Tensor], lead: torch.Size) -> Optional[Tensor]:
-    if valid is None:
-        return None
-    if valid.dtype != torch.bool or valid.shape != lead:
+def _check_valid(valid: Optional[Tensor], lead: torch.Size) -> None:
+    if valid is not None and (valid.dtype != torch.bool or valid.shape != lead):
         raise ValueError(f"valid is a bool tensor of shape {tuple(lead)}, got {valid.dtype} {tuple(valid.shape)}")
-    return valid.reshape(-1)
 
 
 def _check_blocks(num_blocks: int) -> int:
@@ -142,17 +136,16 @@ def block_counts(remote_indices: Tensor, remote_counts: Tensor, num_blocks: int,
     [..., capacity], of which row t's first remote_counts[t] count (ids outside [0, num_blocks) do not);
     ``valid`` (bool [...]) leaves rows out, for example padding."""
     NB = _check_blocks(num_blocks)
-    idx, cnt = _routes(remote_indices, remote_counts)
-    rows = _valid(valid, remote_counts.shape)
-    require_cuda(idx, cnt, rows)
-    _, counts, _ = kernels.balance_loss_fwd(None, idx, cnt, NB, 0, 1.0, rows)
+    _check_routes(remote_indices, remote_counts)
+    _check_valid(valid, remote_counts.shape)
+    _, counts, _ = kernels.balance_loss_fwd(None, remote_indices, remote_counts, NB, 0, 1.0, valid)
     return counts
 
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, scores, idx, cnt, base, temperature, valid, counts_in):
-        loss, counts, state = kernels.balance_loss_fwd(scores, idx, cnt, scores.shape[1], base, temperature, valid,
+        loss, counts, state = kernels.balance_loss_fwd(scores, idx, cnt, scores.shape[-1], base, temperature, valid,
                                                        counts_in)
         ctx.base, ctx.temperature = base, temperature
         ctx.save_for_backward(scores, valid, state)
@@ -189,17 +182,18 @@ def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts
     if not scores.is_floating_point():
         raise TypeError(f"scores must be floating point, got {scores.dtype}")
     lead = scores.shape[:-1]
-    idx = cnt = None
     if counts is not None:
         if counts.dtype != torch.int64 or counts.shape != (NB,):
             raise ValueError(f"counts is an int64 tensor [{NB}], got {counts.dtype} {tuple(counts.shape)}")
+        remote_indices = remote_counts = None
     else:
         if remote_indices is None or remote_counts is None:
             raise ValueError("remote_indices and remote_counts are needed unless counts are given")
-        idx, cnt = _routes(remote_indices, remote_counts)
+        _check_routes(remote_indices, remote_counts)
         if remote_counts.shape != lead:
             raise ValueError(f"routes of {tuple(remote_counts.shape)} rows for scores of {tuple(lead)}")
-    rows = _valid(valid, lead)
-    require_cuda(scores, idx, cnt, rows, counts)
-    return _BalanceLoss.apply(scores.reshape(-1, NB).float(), idx, cnt, int(base_blocks), float(temperature), rows,
-                              counts)
+    _check_valid(valid, lead)
+    require_cuda(scores, remote_indices, remote_counts, valid, counts)
+    if scores.dtype != torch.float32:
+        scores = scores.float()
+    return _BalanceLoss.apply(scores, remote_indices, remote_counts, int(base_blocks), float(temperature), valid, counts)
