@@ -309,5 +309,8 @@ inline cudaError_t launch_pdl(void (*kern)(Exp...), dim3 grid, dim3 block, size_
 // ---- tensor maps
 bool encode_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                    uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
+// Bytes, 64-byte swizzle (box_inner at most 64; row_bytes a multiple of 16).
+bool encode_map_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                      uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
 
 }  // namespace fp

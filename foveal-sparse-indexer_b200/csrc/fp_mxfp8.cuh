@@ -46,6 +46,18 @@ __device__ __forceinline__ float2 mx_unpack2(uint16_t c) {
   return v;
 }
 
+// For blocks that hold a NaN, an infinity or a magnitude near 2^128 (rare): makes v what its code shall stand
+// for, and returns the bits of its magnitude for the block's maximum, 0 where it is not finite.
+__device__ __forceinline__ uint32_t mx_finite(float& v) {
+  const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
+  if (b >= kF32Inf) {
+    v = __uint_as_float(0x7FC00000u);
+    return 0;
+  }
+  if (b >= __float_as_uint(kMxHuge)) v = copysignf(kMxLargest, v);
+  return b;
+}
+
 template <typename T>
 __device__ __forceinline__ T mx_from_f32(float v);
 template <>
@@ -127,15 +139,7 @@ struct MxVec {
     if (__any_sync(0xffffffffu, top >= __float_as_uint(kMxHuge))) {  // rare: NaN, infinity or a value near 2^128
       uint32_t fin = 0;
 #pragma unroll
-      for (int e = 0; e < kV; ++e) {
-        const uint32_t b = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-        if (b >= kF32Inf) {
-          v[e] = __uint_as_float(0x7FC00000u);
-        } else {
-          fin = max(fin, b);
-          if (b >= __float_as_uint(kMxHuge)) v[e] = copysignf(kMxLargest, v[e]);
-        }
-      }
+      for (int e = 0; e < kV; ++e) fin = max(fin, mx_finite(v[e]));
       top = group_max(fin);
     }
     const int byte = mx_scale_byte(top);

@@ -29,18 +29,6 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// ------------------------------------------------------------------ gradient of the scores
-// Three launches.  (1) One pass over dS: dq of every token and partial sums of dK.  (2) One pass over x: dx and
-// partial sums of dWq.  (3) The partial sums, in a fixed order.  The products are 16 wide on one side, so the
-// passes are bound by memory once they run on tensor cores; a tile of 128 rows (tcgen05) would be filled to
-// an eighth, mma.sync fits: the 16 router dimensions are its m (pass 1) and its k or two n-tiles (pass 2).
-//
-// Precision.  Pass 1 multiplies fp32 values as tf32 pieces, v = hi + lo (the rest is below 2^-22 of v):
-// hi hi + hi lo + lo hi, fp32 accumulators.  Pass 2 with bf16 x holds dq as two bf16 pieces (rest below
-// 2^-17 of dq, against 2^-9 for the bf16 gradients), x and Wq are exact.  fp32 x stays on the FMA units.
-//
-// Fragment coordinates below: lane = 4 g + t, g = 0..7, t = 0..3.
-
 __device__ __forceinline__ uint32_t tf32_of(float v) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
@@ -65,6 +53,15 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same from zero accumulators.
+__device__ __forceinline__ void mma_bf16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -75,6 +72,202 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// ------------------------------------------------------------------ scores of the training forward
+// fp_router_scores' bf16 kernel (same products in the same order, so the same bits) for whole batches: a CTA
+// stays for many tiles of 32 tokens, with the block keys in shared memory once (loaded per 16 tokens they took
+// as long as the projection), a key serves four tokens from registers, and the normalisation factor and
+// (kKeep) the MXFP8 copy of x leave in the same pass over x.  Warp: one quarter of D, 16 tokens; then 4
+// tokens' scores.  HBM bound by x.
+constexpr int kFwWarps = 8;
+constexpr int kFwTokens = 32;
+
+// MXFP8 codes of 16 consecutive bf16 values (w: in order); the lane's neighbour (lane ^ 1) holds the other half of
+// the block.  All lanes of the warp call this together.
+__device__ __forceinline__ void mx_quantize16(const uint32_t (&w)[8], uint4& codes, int& byte) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+  uint32_t top = max(m & 0xFFFF0000u, m << 16);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+  if (__any_sync(0xffffffffu, top >= __float_as_uint(kMxHuge))) {
+    uint32_t fin = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) fin = max(fin, mx_finite(v[i]));
+    top = max(fin, __shfl_xor_sync(0xffffffffu, fin, 1));
+  }
+  byte = mx_scale_byte(top);
+  const float inv = mx_inv_scale(byte);
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c[i] = (uint32_t)mx_pack2(v[4 * i] * inv, v[4 * i + 1] * inv) |
+           ((uint32_t)mx_pack2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16);
+  codes = make_uint4(c[0], c[1], c[2], c[3]);
+}
+
+__device__ __forceinline__ void load32(const __nv_bfloat16* p, uint32_t (&w)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
+}
+
+template <bool kKeep>
+__global__ void __launch_bounds__(kFwWarps * 32, 2)
+router_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ wq,
+                  const __nv_bfloat16* __restrict__ k16, int64_t M, int D, int NB, float* __restrict__ scores,
+                  float* __restrict__ q16, float* __restrict__ rnorm, uint8_t* __restrict__ codes,
+                  uint8_t* __restrict__ scales) {
+  extern __shared__ float skeys[];               // [16][NB] block keys
+  __shared__ float sq[2][4][16 * 17];            // [token group][quarter of D] partial projections
+  __shared__ float4 sv[kFwTokens * 4];           // [token][16] projections
+  for (int i = threadIdx.x; i < NB * kIdx; i += blockDim.x) {
+    const int j = i / NB, b = i - j * NB;
+    skeys[i] = __bfloat162float(k16[b * kIdx + j]);
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int quarter = warp & 3, group = warp >> 2, dpart = D / 4, kbeg = quarter * dpart;
+  const __nv_bfloat16* wa = wq + (int64_t)g * D + kbeg + 16 * t;
+  const __nv_bfloat16* wb = wa + (int64_t)8 * D;
+  for (int64_t tok0 = (int64_t)blockIdx.x * kFwTokens; tok0 < M; tok0 += (int64_t)gridDim.x * kFwTokens) {
+    const int64_t ta = tok0 + 16 * group + g, tb = ta + 8;
+    const int64_t oa = (ta < M ? ta : M - 1) * D + kbeg + 16 * t, ob = (tb < M ? tb : M - 1) * D + kbeg + 16 * t;
+    float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k0 = 0; k0 < dpart; k0 += 64) {
+      uint32_t A0[8], A1[8], B0[8], B1[8];
+      load32(x + oa + k0, A0);
+      load32(x + ob + k0, A1);
+      load32(wa + k0, B0);
+      load32(wb + k0, B1);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        mma_bf16(c0, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], B0[2 * st], B0[2 * st + 1]);
+        mma_bf16(c1, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], B1[2 * st], B1[2 * st + 1]);
+      }
+      if constexpr (kKeep) {
+        uint4 q;
+        int byte;
+        mx_quantize16(A0, q, byte);
+        if (ta < M) {
+          *reinterpret_cast<uint4*>(codes + oa + k0) = q;
+          if (!(t & 1)) scales[(oa + k0) / kMxBlock] = (uint8_t)byte;
+        }
+        mx_quantize16(A1, q, byte);
+        if (tb < M) {
+          *reinterpret_cast<uint4*>(codes + ob + k0) = q;
+          if (!(t & 1)) scales[(ob + k0) / kMxBlock] = (uint8_t)byte;
+        }
+      }
+    }
+    float* q = sq[group][quarter];
+    q[g * 17 + 2 * t] = c0[0];
+    q[g * 17 + 2 * t + 1] = c0[1];
+    q[(g + 8) * 17 + 2 * t] = c0[2];
+    q[(g + 8) * 17 + 2 * t + 1] = c0[3];
+    q[g * 17 + 8 + 2 * t] = c1[0];
+    q[g * 17 + 9 + 2 * t] = c1[1];
+    q[(g + 8) * 17 + 8 + 2 * t] = c1[2];
+    q[(g + 8) * 17 + 9 + 2 * t] = c1[3];
+    __syncthreads();
+    // the quarters' sum, in order: two tokens at a time, lane = (token, dimension)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = warp * 4 + 2 * h + (lane >> 4), j = lane & 15, i = (r & 15) * 17 + j;
+      float v = sq[r >> 4][0][i];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) v += sq[r >> 4][w][i];
+      reinterpret_cast<float*>(sv)[r * 16 + j] = v;
+    }
+    __syncwarp();
+    const float eps = 1.1920928955078125e-07f;  // torch.finfo(float32).eps: F.rms_norm's default
+    float qv[4][16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t tok = tok0 + warp * 4 + r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = sv[(warp * 4 + r) * 4 + i];
+        qv[r][4 * i] = v.x; qv[r][4 * i + 1] = v.y; qv[r][4 * i + 2] = v.z; qv[r][4 * i + 3] = v.w;
+      }
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) ss = fmaf(qv[r][j], qv[r][j], ss);
+      const float inv = __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / 16.0f) + eps));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) qv[r][j] *= inv;
+      if (tok < M) {
+        if (lane < 16) q16[tok * 16 + lane] = reinterpret_cast<float*>(sv)[(warp * 4 + r) * 16 + lane] * inv;
+        if (lane == 0) rnorm[tok] = inv;
+      }
+    }
+    float* out = scores + (tok0 + warp * 4) * NB;
+    const int live = (int)min((int64_t)4, M - (tok0 + warp * 4));
+    for (int b = lane; b < NB; b += 32) {
+      float sc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float kv = skeys[j * NB + b];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[r] = fmaf(qv[r][j], kv, sc[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < live) out[(int64_t)r * NB + b] = sc[r] * 0.25f;  // / sqrt(16)
+    }
+    __syncthreads();  // the partial projections' place is free again
+  }
+}
+
+template <bool kKeep>
+int launch_router_fwd(const void* x, const void* wq, const void* k16, int64_t M, int D, int NB, float* scores,
+                      float* q16, float* rnorm, void* codes, void* scales, int sms, cudaStream_t st) {
+  const auto kern = router_fwd_kernel<kKeep>;
+  const size_t smem = (size_t)NB * kIdx * 4;  // at most 64 KB
+  if (smem > 36 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return FP_ERR_CUDA;
+  const int grid = (int)std::min<int64_t>((M + kFwTokens - 1) / kFwTokens, 2 * sms);
+  kern<<<grid, kFwWarps * 32, smem, st>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)k16,
+                                          M, D, NB, scores, q16, rnorm, (uint8_t*)codes, (uint8_t*)scales);
+  return launched();
+}
+
+// ------------------------------------------------------------------ gradient of the scores
+// Three launches.  (1) One pass over dS: dq of every token and partial sums of dK.  (2) One pass over x: dx and
+// partial sums of dWq.  (3) The partial sums, in a fixed order.  The products are 16 wide on one side, so the
+// passes are bound by memory once they run on tensor cores; a tile of 128 rows (tcgen05) would be filled to
+// an eighth, mma.sync fits: the 16 router dimensions are its m (pass 1) and its k or two n-tiles (pass 2).
+//
+// Precision.  Pass 1 multiplies fp32 values as tf32 pieces, v = hi + lo (the rest is below 2^-22 of v):
+// hi hi + hi lo + lo hi, fp32 accumulators.  Pass 2 with bf16 x holds dq as two bf16 pieces (rest below
+// 2^-17 of dq, against 2^-9 for the bf16 gradients), x and Wq are exact.  fp32 x stays on the FMA units.
+//
+// Fragment coordinates below: lane = 4 g + t, g = 0..7, t = 0..3.
+
+// 16 consecutive elements, 16-byte aligned.
+__device__ __forceinline__ void load_row16(const float* p, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p) + i);
+    v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
+  }
+}
+__device__ __forceinline__ void load_row16(const __nv_bfloat16* p, float (&v)[16]) {
+  uint32_t w[8];
+  load32(p, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
 // Four columns of one row of dS, zeros outside.
 __device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, int64_t M, int b, int NB, bool vec) {
   if (t >= M || b >= NB) return make_float4(0.f, 0.f, 0.f, 0.f);
@@ -83,11 +276,11 @@ __device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, i
   return make_float4(p[0], b + 1 < NB ? p[1] : 0.f, b + 2 < NB ? p[2] : 0.f, b + 3 < NB ? p[3] : 0.f);
 }
 
-constexpr int kDqWarps = 4;
-constexpr int kDqTokens = 16 * kDqWarps;  // tokens of a CTA's tile
+constexpr int kDqWarps = 8;
+constexpr int kDqTokens = 8 * kDqWarps;  // tokens of a CTA's tile
 constexpr int kDqMaxCtas = 296;
 
-// Pass 1.  Phase A, 16 tokens to a warp: a^T[j, tok] = K^T[j, b] dS^T[b, tok], then dq.  Phase B, a share of
+// Pass 1.  Phase A, 8 tokens to a warp: a^T[j, tok] = K^T[j, b] dS^T[b, tok], then dq.  Phase B, a share of
 // the blocks (kG groups of 32) to a warp, over the CTA's 64 tokens (rows just read, from L1): dK^T[j, b] =
 // n^T[j, tok] dS[tok, b], kept in registers over all of the CTA's tiles.  The order of b within a product and
 // the columns of a tile are permuted so that a lane's elements are 16 contiguous bytes.
@@ -104,18 +297,20 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
   const int nk = (NB + 15) / 16;
   const bool vec = (NB & 3) == 0;
   if (dq_out) {
-    for (int i = threadIdx.x; i < nk * 64; i += blockDim.x) {
-      const int l = i & 31, s = (i >> 5) & 1, b = (i >> 6) * 16 + 4 * (l & 3) + 2 * s, j = l >> 2;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (b < NB) {
-        v.x = to_f32(k16[b * kIdx + j]);
-        v.y = to_f32(k16[b * kIdx + j + 8]);
-      }
-      if (b + 1 < NB) {
-        v.z = to_f32(k16[(b + 1) * kIdx + j]);
-        v.w = to_f32(k16[(b + 1) * kIdx + j + 8]);
-      }
-      sk[i] = v;
+    // the first tile's rows start towards L2 while K goes to shared memory, one row of K to a thread
+    const int64_t row0 = (int64_t)blockIdx.x * kDqTokens + 8 * warp;
+    const int64_t bytes = min((int64_t)8, M - row0) * NB * 4;
+    for (int64_t o = 128 * lane; o < bytes; o += 4096)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(ds + row0 * NB) + o));
+    for (int b = threadIdx.x; b < nk * 16; b += blockDim.x) {
+      float v[kIdx];
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) v[j] = 0.f;
+      if (b < NB) load_row16(k16 + b * kIdx, v);
+      // row b is k-index t (even) or t + 4 (odd) of step s: t = b / 4 % 4, s = b / 2 % 2
+      float* o = reinterpret_cast<float*>(sk) + (((b >> 4) * 2 + (b >> 1 & 1)) * 32 + (b >> 2 & 3)) * 4 + 2 * (b & 1);
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) o[16 * (j & 7) + (j >> 3)] = v[j];
     }
     __syncthreads();
   }
@@ -128,14 +323,24 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
       for (int e = 0; e < 4; ++e) dk[i][k][e] = 0.f;
 
   for (int64_t base = (int64_t)blockIdx.x * kDqTokens; base < M; base += (int64_t)gridDim.x * kDqTokens) {
-    const int64_t tok0 = base + 16 * warp;
-    if (dq_out && tok0 < M) {
-      float c[2][4] = {};
-#pragma unroll 2
-      for (int k = 0; k < nk; ++k) {
-        float4 v[2];
+    const int64_t tok0 = base + 8 * warp;
+    // (a tile of 16 tokens that ends past M is written whole: zeros behind the last token)
+    if (dq_out && tok0 < (M + 15) / 16 * 16) {
+      float c[4] = {}, cl[4] = {};
+      float n0[2], n1[2], r[2];  // of tokens 2 t and 2 t + 1
 #pragma unroll
-        for (int n = 0; n < 2; ++n) v[n] = ds4(ds, tok0 + 8 * n + g, M, 16 * k + 4 * t, NB, vec);
+      for (int e = 0; e < 2; ++e) {
+        const int64_t tok = tok0 + 2 * t + e;
+        n0[e] = n1[e] = r[e] = 0.f;
+        if (tok < M) {
+          n0[e] = __ldg(q16 + tok * kIdx + g);
+          n1[e] = __ldg(q16 + tok * kIdx + g + 8);
+          r[e] = __ldg(rnorm + tok);
+        }
+      }
+#pragma unroll 8
+      for (int k = 0; k < nk; ++k) {
+        const float4 v = ds4(ds, tok0 + g, M, 16 * k + 4 * t, NB, vec);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const float4 kv = sk[(k * 2 + s) * 32 + lane];
@@ -146,61 +351,51 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
             if constexpr (sizeof(T) == 4) tf32_split(kf[e], kh[e], kl[e]);
             else kh[e] = __float_as_uint(kf[e]);  // a bf16 value is a tf32 value
           }
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            uint32_t h0, l0, h1, l1;
-            tf32_split(s ? v[n].z : v[n].x, h0, l0);
-            tf32_split(s ? v[n].w : v[n].y, h1, l1);
-            mma_tf32(c[n], kh, l0, l1);
-            if constexpr (sizeof(T) == 4) mma_tf32(c[n], kl, h0, h1);
-            mma_tf32(c[n], kh, h0, h1);
-          }
+          uint32_t h0, l0, h1, l1;
+          tf32_split(s ? v.z : v.x, h0, l0);
+          tf32_split(s ? v.w : v.y, h1, l1);
+          mma_tf32(cl, kh, l0, l1);
+          if constexpr (sizeof(T) == 4) mma_tf32(cl, kl, h0, h1);
+          mma_tf32(c, kh, h0, h1);
         }
       }
-      // c[n]: token 8 n + 2 t (+1: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
-      uint32_t hi[2][2], lo[2][2];
+      // c: token 2 t (+1: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
+      float d[2][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float d[2][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int64_t tok = tok0 + 8 * n + 2 * t + e;
-          const bool in = tok < M;
-          const float n0 = in ? q16[tok * kIdx + g] : 0.f, n1 = in ? q16[tok * kIdx + g + 8] : 0.f;
-          const float a0 = c[n][e] * 0.25f, a1 = c[n][2 + e] * 0.25f;
-          float dot = a0 * n0 + a1 * n1;
-          dot += __shfl_xor_sync(0xffffffffu, dot, 4);
-          dot += __shfl_xor_sync(0xffffffffu, dot, 8);
-          dot += __shfl_xor_sync(0xffffffffu, dot, 16);
-          dot *= 1.0f / kIdx;
-          const float r = in ? rnorm[tok] : 0.f;
-          d[0][e] = in ? r * (a0 - n0 * dot) : 0.f;
-          d[1][e] = in ? r * (a1 - n1 * dot) : 0.f;
-          if constexpr (!kPacked) {
-            if (in) {
-              float* o = reinterpret_cast<float*>(dq_out) + tok * kIdx + g;
-              o[0] = d[0][e];
-              o[8] = d[1][e];
-            }
-          }
-        }
-        if constexpr (kPacked) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t h = pack_bf16(d[j][0], d[j][1]);
-            hi[n][j] = h;
-            lo[n][j] = pack_bf16(d[j][0] - __uint_as_float(h << 16), d[j][1] - __uint_as_float(h & 0xFFFF0000u));
+      for (int e = 0; e < 2; ++e) {
+        const int64_t tok = tok0 + 2 * t + e;
+        const bool in = tok < M;
+        const float a0 = (c[e] + cl[e]) * 0.25f, a1 = (c[2 + e] + cl[2 + e]) * 0.25f;
+        float dot = a0 * n0[e] + a1 * n1[e];
+        dot += __shfl_xor_sync(0xffffffffu, dot, 4);
+        dot += __shfl_xor_sync(0xffffffffu, dot, 8);
+        dot += __shfl_xor_sync(0xffffffffu, dot, 16);
+        dot *= 1.0f / kIdx;
+        d[0][e] = in ? r[e] * (a0 - n0[e] * dot) : 0.f;
+        d[1][e] = in ? r[e] * (a1 - n1[e] * dot) : 0.f;
+        if constexpr (!kPacked) {
+          if (in) {
+            float* o = reinterpret_cast<float*>(dq_out) + tok * kIdx + g;
+            o[0] = d[0][e];
+            o[8] = d[1][e];
           }
         }
       }
       if constexpr (kPacked) {
-        uint4* o = reinterpret_cast<uint4*>(dq_out) + (tok0 / 16) * 64 + lane;
-        o[0] = make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
-        o[32] = make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          hi[j] = pack_bf16(d[j][0], d[j][1]);
+          lo[j] = pack_bf16(d[j][0] - __uint_as_float(hi[j] << 16), d[j][1] - __uint_as_float(hi[j] & 0xFFFF0000u));
+        }
+        uint2* o = reinterpret_cast<uint2*>(dq_out) + (tok0 / 16) * 128 + 2 * lane + (tok0 / 8 & 1);
+        o[0] = make_uint2(hi[0], hi[1]);
+        o[64] = make_uint2(lo[0], lo[1]);
       }
     }
     if (dk_part) {
       const int64_t end = min(base + kDqTokens, M);
+#pragma unroll (kG == 1 ? 4 : kG == 2 ? 2 : 1)
       for (int64_t s0 = base; s0 < end; s0 += 8) {
         const int64_t ta = s0 + t, tb = s0 + t + 4;
         uint32_t nh[4], nl[4];
@@ -248,49 +443,34 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
 // the token groups' dWq are joined in shared memory, in order.
 constexpr int kXWarps = 8;
 
+// x (or its codes) comes by TMA, 64 columns x 16 tokens a tile, and dq with it, into a ring of kXStages tiles that a
+// warp keeps for itself: one lane copies, every lane waits on the stage's mbarrier, no other barrier.  Rows
+// and columns past the end arrive as zeros.
+constexpr int kXStages = 4;
 template <bool kCodes>
-struct XRows {
-  uint4 r[4];
-  __device__ __forceinline__ void load(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__ codes,
-                                       const uint8_t* __restrict__ scales, int64_t tok0, int64_t M, int D, int d, int t) {
-    uint2 c[4];
-    uint32_t byte[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t tok = tok0 + 2 * t + (k & 1) + 8 * (k >> 1);
-      const bool in = tok < M && d < D;
-      const int64_t i = tok * D + d;
-      if constexpr (kCodes) {
-        c[k] = in ? __ldg(reinterpret_cast<const uint2*>(codes + i)) : make_uint2(0, 0);
-        byte[k] = in ? __ldg(scales + i / kMxBlock) : 127u;
-      } else {
-        r[k] = in ? __ldg(reinterpret_cast<const uint4*>(x + i)) : make_uint4(0, 0, 0, 0);
-      }
-    }
-    if constexpr (kCodes) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float s = mx_scale((int)byte[k]);
-        const float2 a = mx_unpack2((uint16_t)c[k].x), b = mx_unpack2((uint16_t)(c[k].x >> 16));
-        const float2 e = mx_unpack2((uint16_t)c[k].y), f = mx_unpack2((uint16_t)(c[k].y >> 16));
-        r[k] = make_uint4(pack_bf16(a.x * s, a.y * s), pack_bf16(b.x * s, b.y * s), pack_bf16(e.x * s, e.y * s),
-                          pack_bf16(f.x * s, f.y * s));
-      }
-    }
-  }
-};
+constexpr int kXTileBytes = kCodes ? 1024 : 2048;
+template <bool kCodes>
+constexpr int kXSmem = kXWarps * kXStages * (kXTileBytes<kCodes> + 1024 + 8) + 1024;
 
 template <bool kCodes>
 __global__ void __launch_bounds__(kXWarps * 32, 2)
-router_x_kernel(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__ codes,
-                const uint8_t* __restrict__ scales, const uint4* __restrict__ dq, const __nv_bfloat16* __restrict__ wq,
-                int64_t M, int D, int wd, int64_t tiles_per_cta, __nv_bfloat16* __restrict__ dx,
-                float* __restrict__ dw_part) {
-  __shared__ float red[kXWarps * 64 * kIdx];  // [token group][j][wd * 64]
+router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restrict__ scales,
+                const uint4* __restrict__ dq, const __nv_bfloat16* __restrict__ wq, int64_t M, int D, int wd,
+                __nv_bfloat16* __restrict__ dx, float* __restrict__ dw_part) {
+  extern __shared__ uint8_t dyn[];
+  // [warp][stage] tiles of x, [warp][stage] tiles of dq, [warp][stage] barriers; at the end red[token group][j][wd * 64]
+  uint8_t* ring = dyn + (1024 - (smem_u32(dyn) & 1023)) % 1024;  // the swizzle counts from 1024-byte boundaries
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int dw = warp % wd, tw = warp / wd, ntw = kXWarps / wd;
   const int d0 = (blockIdx.x * wd + dw) * 64, dl = d0 + 8 * g;
+  uint8_t* xs = ring + warp * kXStages * kXTileBytes<kCodes>;
+  uint8_t* qs = ring + kXWarps * kXStages * kXTileBytes<kCodes> + warp * kXStages * 1024;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kXWarps * kXStages * (kXTileBytes<kCodes> + 1024)) + warp * kXStages;
+  if (lane == 0) {
+    for (int k = 0; k < kXStages; ++k) mbar_init(bars + k, 1);
+    fence_mbar_init();
+  }
   uint32_t wb[8][2];
   if (dx) {
 #pragma unroll
@@ -312,38 +492,86 @@ router_x_kernel(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-  const int64_t tiles = (M + 15) / 16;
-  const int64_t tile1 = min((int64_t)(blockIdx.y + 1) * tiles_per_cta, tiles);
+  const int tiles = d0 < D ? (int)((M + 15) / 16) : 0;
+  const int tile0 = blockIdx.y * ntw + tw, hop = gridDim.y * ntw;
+  const auto fetch = [&](int tile, int stage) {  // lane 0
+    if (tile >= tiles) return;
+    mbar_arrive_expect_tx(bars + stage, dw_part ? kXTileBytes<kCodes> + 1024 : 1024);
+    if (dw_part) tma_load_2d(xs + stage * kXTileBytes<kCodes>, &map, bars + stage, d0, tile * 16);
+    bulk_load(qs + stage * 1024, dq + (int64_t)tile * 64, 1024, bars + stage);
+  };
+  uint32_t byte[4] = {127u, 127u, 127u, 127u};
+  int64_t at = ((int64_t)tile0 * 16 + 2 * t) * D + dl;  // element that the next scales belong to
+  const auto fetch_scales = [&](int tile) {
+    if constexpr (kCodes) {
+      if (dw_part && dl < D && tile < tiles) {
+        const bool whole = (int64_t)tile * 16 + 16 <= M;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = (k & 1) + 8 * (k >> 1);
+          if (whole || (int64_t)tile * 16 + 2 * t + r < M) byte[k] = __ldg(scales + ((at + (int64_t)r * D) >> 5));
+        }
+      }
+      at += (int64_t)16 * hop * D;
+    }
+  };
+  __nv_bfloat16* po = dx + ((int64_t)tile0 * 16 + g) * D + d0 + 8 * t;
+  const bool out0 = d0 + 8 * t < D, out1 = d0 + 32 + 8 * t < D;
+
+  fetch_scales(tile0);
   griddep_wait();
-  for (int64_t tile = (int64_t)blockIdx.y * tiles_per_cta + tw; tile < tile1; tile += ntw) {
-    XRows<kCodes> xr;
-    if (dw_part) xr.load(x, codes, scales, tile * 16, M, D, dl, t);
-    const uint4 h4 = __ldg(dq + tile * 64 + lane), l4 = __ldg(dq + tile * 64 + 32 + lane);
+  if (lane == 0)
+    for (int k = 0; k < kXStages; ++k) fetch(tile0 + k * hop, k);
+  __syncwarp();  // the barriers' initialisation
+  int stage = 0, tile = tile0;
+  uint32_t parity = 0;
+  for (; tile < tiles; tile += hop) {
+    if (!mbar_wait(bars + stage, parity, nullptr, 0)) break;
+    const uint4* q = reinterpret_cast<const uint4*>(qs + stage * 1024);
+    const uint4 h4 = q[lane], l4 = q[32 + lane];
+    uint4 r[4];
+    if (dw_part) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = 2 * t + (k & 1) + 8 * (k >> 1);
+        if constexpr (kCodes) {  // 64-byte swizzle: 16-byte piece ^ (row / 2) % 4
+          const uint2 c = *reinterpret_cast<const uint2*>(xs + stage * 1024 + row * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8);
+          const float f = mx_scale((int)byte[k]);
+          const float2 a = mx_unpack2((uint16_t)c.x), b = mx_unpack2((uint16_t)(c.x >> 16));
+          const float2 e = mx_unpack2((uint16_t)c.y), z = mx_unpack2((uint16_t)(c.y >> 16));
+          r[k] = make_uint4(pack_bf16(a.x * f, a.y * f), pack_bf16(b.x * f, b.y * f), pack_bf16(e.x * f, e.y * f),
+                            pack_bf16(z.x * f, z.y * f));
+        } else {  // 128-byte swizzle: 16-byte piece ^ row % 8
+          r[k] = *reinterpret_cast<const uint4*>(xs + stage * 2048 + row * 128 + ((g ^ (row & 7)) << 4));
+        }
+      }
+    }
+    fetch_scales(tile + hop);
     if (dx) {
       const uint32_t ah[4] = {transpose8x8(h4.x), transpose8x8(h4.z), transpose8x8(h4.y), transpose8x8(h4.w)};
       const uint32_t al[4] = {transpose8x8(l4.x), transpose8x8(l4.z), transpose8x8(l4.y), transpose8x8(l4.w)};
-      const int64_t ra = tile * 16 + g, rb = ra + 8;
+      const bool in_a = (int64_t)tile * 16 + g < M, in_b = (int64_t)tile * 16 + 8 + g < M;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t oa[4], ob[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_bf16(c, al[0], al[1], al[2], al[3], wb[4 * h + i][0], wb[4 * h + i][1]);
+          float c[4];
+          mma_bf16_zero(c, al[0], al[1], al[2], al[3], wb[4 * h + i][0], wb[4 * h + i][1]);
           mma_bf16(c, ah[0], ah[1], ah[2], ah[3], wb[4 * h + i][0], wb[4 * h + i][1]);
           oa[i] = pack_bf16(c[0], c[1]);
           ob[i] = pack_bf16(c[2], c[3]);
         }
-        const int d = d0 + 32 * h + 8 * t;
-        if (d < D) {
-          if (ra < M) *reinterpret_cast<uint4*>(dx + ra * D + d) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-          if (rb < M) *reinterpret_cast<uint4*>(dx + rb * D + d) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+        if (h ? out1 : out0) {
+          if (in_a) *reinterpret_cast<uint4*>(po + 32 * h) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+          if (in_b) *reinterpret_cast<uint4*>(po + 32 * h + 8 * D) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
         }
       }
+      po += (int64_t)16 * hop * D;
     }
     if (dw_part) {
-      const uint32_t w0[4] = {xr.r[0].x, xr.r[0].y, xr.r[0].z, xr.r[0].w}, w1[4] = {xr.r[1].x, xr.r[1].y, xr.r[1].z, xr.r[1].w};
-      const uint32_t w2[4] = {xr.r[2].x, xr.r[2].y, xr.r[2].z, xr.r[2].w}, w3[4] = {xr.r[3].x, xr.r[3].y, xr.r[3].z, xr.r[3].w};
+      const uint32_t w0[4] = {r[0].x, r[0].y, r[0].z, r[0].w}, w1[4] = {r[1].x, r[1].y, r[1].z, r[1].w};
+      const uint32_t w2[4] = {r[2].x, r[2].y, r[2].z, r[2].w}, w3[4] = {r[3].x, r[3].y, r[3].z, r[3].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a0 = __byte_perm(w0[i], w1[i], 0x5410), a1 = __byte_perm(w0[i], w1[i], 0x7632);
@@ -354,10 +582,41 @@ router_x_kernel(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__
         mma_bf16(acc[i][1], a0, a1, a2, a3, h4.y, h4.w);
       }
     }
+    __syncwarp();  // the tile is in every lane's registers: its place takes the tile kXStages on
+    if (lane == 0) fetch(tile + kXStages * hop, stage);
+    if (++stage == kXStages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+  if (tile < tiles) {  // a copy did not arrive within the wait limit: drain the others, leave NaN as the result
+    for (int k = 1; k < kXStages; ++k) {
+      if (++stage == kXStages) {
+        stage = 0;
+        parity ^= 1;
+      }
+      if (tile + k * hop < tiles) mbar_wait(bars + stage, parity, nullptr, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __uint_as_float(0x7FC00000u);
+    for (; dx && tile < tiles; tile += hop) {
+      const uint32_t n = 0x7FC07FC0u;
+      for (int k = 0; k < 4; ++k) {
+        const int64_t row = (int64_t)tile * 16 + g + 8 * (k & 1);
+        if (row < M && (k < 2 ? out0 : out1))
+          *reinterpret_cast<uint4*>(dx + row * D + d0 + 8 * t + (k < 2 ? 0 : 32)) = make_uint4(n, n, n, n);
+      }
+    }
   }
   if (!dw_part) return;
   // acc[i][j]: column 8 g + 2 i (elements 0, 1) and + 1 (2, 3), dimension 8 j + 2 t (+1: odd element)
   const int width = wd * 64;
+  float* red = reinterpret_cast<float*>(ring);
+  __syncthreads();  // every warp is through with its ring
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -378,9 +637,18 @@ router_x_kernel(const __nv_bfloat16* __restrict__ x, const uint8_t* __restrict__
 
 // Pass 2, fp32, on the FMA units (32 per element): a thread owns 4 columns (their Wq and dWq in registers),
 // dq of 32 tokens at a time in shared memory; tx threads (32, 64, 128) lie along the columns, 128 / tx along
-// tokens.
+// tokens.  x runs through a ring of kFAhead tokens that a thread keeps for itself (cp.async; with two loads
+// in flight from registers the pass took 238 us at 16384 x 4096).
 constexpr int kFThreads = 128;
 constexpr int kFTokens = 32;
+constexpr int kFAhead = 8;
+
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <bool kCodes>
 __global__ void __launch_bounds__(kFThreads, 3)
@@ -388,7 +656,7 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
                     const float* __restrict__ dq, const float* __restrict__ wq, int64_t M, int D, int tx,
                     int64_t tokens_per_cta, float* __restrict__ dx, float* __restrict__ dw_part) {
   __shared__ float4 sq[kFTokens * 4];
-  __shared__ float red[kFThreads * 4 * kIdx];
+  __shared__ float red[kFThreads * 4 * kIdx];  // during the pass its first half is the ring [kFAhead][thread] float4
   griddep_launch_dependents();
   const int lane = threadIdx.x % tx, ty = threadIdx.x / tx, nty = kFThreads / tx;
   const int d = (blockIdx.x * tx + lane) * 4;
@@ -402,6 +670,25 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
     for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
   }
   const int64_t t1 = min((int64_t)(blockIdx.y + 1) * tokens_per_cta, M);
+  const uint32_t ring = smem_u32(red) + threadIdx.x * 16;
+  // the thread's n-th token from the CTA's first: ty + n nty
+  const int64_t first = (int64_t)blockIdx.y * tokens_per_cta + ty;
+  const auto fetch = [&](int64_t tok, int slot) {
+    if (in && dw_part && tok < t1) {
+      if constexpr (kCodes) cp_async4(ring + slot * kFThreads * 16, codes + tok * D + d);
+      else cp_async_16(ring + slot * kFThreads * 16, x + tok * D + d);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < kFAhead - 1; ++k) fetch(first + (int64_t)k * nty, k);
+  int slot = 0;
+  uint32_t byte = 127u;
+  const auto fetch_scale = [&](int64_t tok) {
+    if constexpr (kCodes)
+      if (in && dw_part && tok < t1) byte = __ldg(scales + (tok * D + d) / kMxBlock);
+  };
+  fetch_scale(first);
   griddep_wait();
   for (int64_t t0 = (int64_t)blockIdx.y * tokens_per_cta; t0 < t1; t0 += kFTokens) {
     const int n = (int)min((int64_t)kFTokens, t1 - t0);
@@ -413,14 +700,19 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
     for (int k = ty; k < n; k += nty) {
       const int64_t i = (t0 + k) * D + d;
       float v[4] = {0.f, 0.f, 0.f, 0.f};
+      cp_async_wait<kFAhead - 2>();
+      const float4* mine = reinterpret_cast<const float4*>(red) + slot * kFThreads + threadIdx.x;
+      fetch(t0 + k + (int64_t)(kFAhead - 1) * nty, slot == 0 ? kFAhead - 1 : slot - 1);
+      slot = slot == kFAhead - 1 ? 0 : slot + 1;
       if (dw_part) {
         if constexpr (kCodes) {
-          const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes + i));
-          const float s = mx_scale((int)__ldg(scales + i / kMxBlock));
+          const uint32_t c = *reinterpret_cast<const uint32_t*>(mine);
+          const float s = mx_scale((int)byte);
+          fetch_scale(t0 + k + nty);
           const float2 a = mx_unpack2((uint16_t)c), b = mx_unpack2((uint16_t)(c >> 16));
           v[0] = a.x * s; v[1] = a.y * s; v[2] = b.x * s; v[3] = b.y * s;
         } else {
-          const float4 q = __ldg(reinterpret_cast<const float4*>(x + i));
+          const float4 q = *mine;
           v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
         }
       }
@@ -440,8 +732,10 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
       if (dx) *reinterpret_cast<float4*>(dx + i) = make_float4(o[0], o[1], o[2], o[3]);
     }
   }
+  cp_async_wait<0>();
   if (!dw_part) return;
   const int width = tx * 4;
+  __syncthreads();  // the ring's place takes the sums
 #pragma unroll
   for (int j = 0; j < kIdx; ++j)
 #pragma unroll
@@ -472,7 +766,7 @@ sum_partials_kernel(const float* __restrict__ p1, int parts1, int64_t n1, T* __r
   griddep_wait();
   float v = 0.f;
   if (i < n) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = row; k < parts; k += 8) v += p[k * n + i];
   }
   s[row][lane] = v;
@@ -489,7 +783,7 @@ sum_partials_kernel(const float* __restrict__ p1, int parts1, int64_t n1, T* __r
 struct BwdPlan {
   int dq_ctas, wide, col_ctas, parts;
   int64_t per_cta;  // pass 2: tiles of 16 tokens (bf16) or tokens (fp32)
-  size_t dq, dw, dk, total;
+  size_t dq, dw, dk, copy, total;
 };
 BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
   BwdPlan p{};
@@ -513,7 +807,8 @@ BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
   p.dq = 0;
   p.dw = p.dq + up((size_t)((M + 15) / 16) * 1024);
   p.dk = p.dw + up((size_t)p.parts * kIdx * D * 4);
-  p.total = p.dk + up((size_t)p.dq_ctas * kIdx * NB * 4);
+  p.copy = p.dk + up((size_t)p.dq_ctas * kIdx * NB * 4);
+  p.total = p.copy + (dtype == FP_DTYPE_BF16 && D % 16 ? up((size_t)M * D * 2) : 0);
   return p;
 }
 
@@ -538,17 +833,30 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
   float* pw = dwq ? reinterpret_cast<float*>(ws + p.dw) : nullptr;
   float* pk = dk16 ? reinterpret_cast<float*>(ws + p.dk) : nullptr;
   int rc;
-  if (NB <= 128) rc = launch_dq<T, 1>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
-  else if (NB <= 256) rc = launch_dq<T, 2>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
-  else if (NB <= 512) rc = launch_dq<T, 4>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
-  else rc = launch_dq<T, 8>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  if (NB <= 256) rc = launch_dq<T, 1>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  else if (NB <= 512) rc = launch_dq<T, 2>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
+  else rc = launch_dq<T, 4>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
   if (rc) return rc;
   if (dq) {
     const dim3 grid(p.col_ctas, p.parts);
     cudaError_t e;
-    if constexpr (sizeof(T) == 2)
-      e = launch_pdl(codes ? router_x_kernel<true> : router_x_kernel<false>, grid, kXWarps * 32, 0, st, x, codes, scales,
-                     (const uint4*)dq, wq, M, D, p.wide, p.per_cta, dx, pw);
+    if constexpr (sizeof(T) == 2) {
+      static_assert(kXSmem<true> >= kXWarps * 64 * kIdx * 4 + 1024, "the ring's place takes the sums");
+      const __nv_bfloat16* rows = x;
+      if (codes && D % 16) {  // rows of codes that TMA cannot address: as bf16 in the workspace
+        rows = reinterpret_cast<const __nv_bfloat16*>(ws + p.copy);
+        if (const int e2 = dwq ? fp_mxfp8_dequantize(codes, scales, FP_DTYPE_BF16, M * D, ws + p.copy, st) : FP_OK) return e2;
+        codes = nullptr;
+      }
+      const auto kern = codes ? router_x_kernel<true> : router_x_kernel<false>;
+      const int smem = codes ? kXSmem<true> : kXSmem<false>;
+      CUtensorMap map{};
+      if (dwq && !(codes ? encode_map_2d_u8(&map, codes, D, M, D, 64, 16)
+                         : encode_map_2d(&map, rows, D, M, (uint64_t)D * 2, 64, 16)))
+        return FP_ERR_CUDA;
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return FP_ERR_CUDA;
+      e = launch_pdl(kern, grid, kXWarps * 32, smem, st, map, scales, (const uint4*)dq, wq, M, D, p.wide, dx, pw);
+    }
     else
       e = launch_pdl(codes ? router_x_f32_kernel<true> : router_x_f32_kernel<false>, grid, kFThreads, 0, st, x, codes,
                      scales, (const float*)dq, wq, M, D, p.wide, p.per_cta, dx, pw);
@@ -1022,8 +1330,11 @@ int fp_router_scores_train(const void* x, const void* q_proj, const void* block_
   if (!al16(x) || !al16(q_proj) || !al16(codes)) return FP_ERR_INVALID_ARG;
   int sms;
   if (const int rc = device_info(sms)) return rc;
-  if (const int rc = launch_router_scores(x, q_proj, block_keys, dtype, M, D, NB, 1.0f, scores, q16,
-                                          (cudaStream_t)stream, nullptr, rnorm))
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == FP_DTYPE_BF16 && D % 256 == 0)
+    return codes ? launch_router_fwd<true>(x, q_proj, block_keys, M, D, NB, scores, q16, rnorm, codes, scales, sms, st)
+                 : launch_router_fwd<false>(x, q_proj, block_keys, M, D, NB, scores, q16, rnorm, codes, scales, sms, st);
+  if (const int rc = launch_router_scores(x, q_proj, block_keys, dtype, M, D, NB, 1.0f, scores, q16, st, nullptr, rnorm))
     return rc;
   return codes ? fp_mxfp8_quantize(x, dtype, M * D, codes, scales, stream) : FP_OK;
 }
@@ -1043,7 +1354,8 @@ int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes,
   if (!dscores || !q_proj || !block_keys || !q16 || !rnorm || !workspace) return FP_ERR_INVALID_ARG;
   if (dq_proj && !x && !codes) return FP_ERR_INVALID_ARG;
   if ((codes == nullptr) != (scales == nullptr)) return FP_ERR_INVALID_ARG;
-  if (!al16(x) || !al16(codes) || !al16(q_proj) || !al16(dx) || !al16(dscores) || !al16(q16) || !al16(workspace))
+  if (!al16(x) || !al16(codes) || !al16(q_proj) || !al16(block_keys) || !al16(dx) || !al16(dscores) || !al16(q16) ||
+      !al16(workspace))
     return FP_ERR_INVALID_ARG;
   if (workspace_bytes < bwd_plan(dtype, M, D, NB).total) return FP_ERR_WORKSPACE;
   int sms;

@@ -161,7 +161,7 @@ def test_c_router(lib):
     assert go(c=A) == INVALID             # codes without scales
     for name in ("ds", "wq", "k", "q", "r", "ws"):
         assert go(**{name: None}) == INVALID, name
-    for name in ("ds", "x", "wq", "q", "dx", "ws"):
+    for name in ("ds", "x", "wq", "k", "q", "dx", "ws"):
         assert go(**{name: ODD}) == INVALID, name
 
 
