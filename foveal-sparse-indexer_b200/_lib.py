@@ -7,7 +7,6 @@ or a non-sm_100 device raises instead of silently computing elsewhere.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -171,9 +170,9 @@ def require_cuda(*tensors: Optional[torch.Tensor]) -> torch.device:
     return dev
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current device (launches go to the current device's streams)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def elsewhere(device: torch.device) -> bool:
+    """Whether another device than ``device`` is the current one (launches go to the current device)."""
+    return torch.cuda.current_device() != device.index
 
 
 def raw_stream(device: torch.device) -> int:

@@ -14,6 +14,7 @@
 #include "fp_mxfp8.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace fp {
 namespace {
@@ -22,6 +23,19 @@ constexpr int kIdx = 16;  // the router's width
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int launched() { return cudaGetLastError() == cudaSuccess ? FP_OK : FP_ERR_CUDA; }
+
+// Lets `kern` use up to `bytes` of dynamic shared memory on the current device (asked for once per device).
+template <auto kern>
+bool allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -227,11 +241,9 @@ router_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __re
 template <bool kKeep>
 int launch_router_fwd(const void* x, const void* wq, const void* k16, int64_t M, int D, int NB, float* scores,
                       float* q16, float* rnorm, void* codes, void* scales, int sms, cudaStream_t st) {
-  const auto kern = router_fwd_kernel<kKeep>;
+  constexpr auto kern = router_fwd_kernel<kKeep>;
   const size_t smem = (size_t)NB * kIdx * 4;  // at most 64 KB
-  if (smem > 36 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return FP_ERR_CUDA;
+  if (smem > 36 * 1024 && !allow_smem<kern>(64 * 1024)) return FP_ERR_CUDA;
   const int grid = (int)std::min<int64_t>((M + kFwTokens - 1) / kFwTokens, 2 * sms);
   kern<<<grid, kFwWarps * 32, smem, st>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)k16,
                                           M, D, NB, scores, q16, rnorm, (uint8_t*)codes, (uint8_t*)scales);
@@ -815,11 +827,9 @@ BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
 template <typename T, int kG>
 int launch_dq(const BwdPlan& p, const float* ds, const T* k16, const float* q16, const float* rnorm, int64_t M, int NB,
               void* dq, float* pk, cudaStream_t st) {
-  const auto kern = router_dq_kernel<T, kG, sizeof(T) == 2>;
+  constexpr auto kern = router_dq_kernel<T, kG, sizeof(T) == 2>;
   const size_t smem = dq ? (size_t)((NB + 15) / 16) * 1024 : 0;  // at most 64 KB
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return FP_ERR_CUDA;
+  if (smem > 48 * 1024 && !allow_smem<kern>(64 * 1024)) return FP_ERR_CUDA;
   kern<<<p.dq_ctas, kDqWarps * 32, smem, st>>>(ds, k16, q16, rnorm, M, NB, dq, pk);
   return launched();
 }
@@ -854,7 +864,7 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
       if (dwq && !(codes ? encode_map_2d_u8(&map, codes, D, M, D, 64, 16)
                          : encode_map_2d(&map, rows, D, M, (uint64_t)D * 2, 64, 16)))
         return FP_ERR_CUDA;
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return FP_ERR_CUDA;
+      if (!(codes ? allow_smem<router_x_kernel<true>>(smem) : allow_smem<router_x_kernel<false>>(smem))) return FP_ERR_CUDA;
       e = launch_pdl(kern, grid, kXWarps * 32, smem, st, map, scales, (const uint4*)dq, wq, M, D, p.wide, dx, pw);
     }
     else
@@ -1271,11 +1281,9 @@ template <int kE, bool kVec>
 int balance_fwd_go(const float* scores, int64_t M, int NB, int base, float temperature, const uint8_t* valid,
                    const int32_t* idx, const int32_t* cnt, int capacity, float* psum, int32_t* rows, int32_t* hist,
                    cudaStream_t st) {
-  const auto kern = balance_partial_kernel<kE, kVec>;
+  constexpr auto kern = balance_partial_kernel<kE, kVec>;
   const size_t smem = (size_t)(kBalWarps + 2) * NB * 4;  // at most 72 KB
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return FP_ERR_CUDA;
+  if (smem > 48 * 1024 && !allow_smem<kern>(72 * 1024)) return FP_ERR_CUDA;
   kern<<<balance_ctas(M), kBalWarps * 32, smem, st>>>(scores, M, NB, base, temperature, valid, idx, cnt, capacity,
                                                       psum, rows, hist);
   return launched();

@@ -29,7 +29,6 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import kernels
-from ._lib import on_device
 from .training import balance_loss, check_checkpoint, router_scores
 
 
@@ -335,7 +334,7 @@ class FovealPattentionMLP(nn.Module):
         scores = router_scores(xx, self.q_proj_16d.weight, self.block_keys_16d, checkpoint=self.checkpoint)
         s2d = scores.detach().reshape(-1, self.num_blocks)
         cap = max(int(self.max_remote_blocks), 1)
-        with on_device(s2d.device):
+        with torch.cuda.device(s2d.device):
             idx, cnt, _, _ = kernels.select(s2d, base_blocks=self.base_blocks, top_p=self.top_p,
                                             min_remote=self.min_remote_blocks, max_remote=self.max_remote_blocks,
                                             capacity=cap, temperature=self.temperature)

@@ -147,8 +147,10 @@ def swiglu_fwd(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
 # Training operators: MXFP8 activation copies, router score gradient, load balance
 # ---------------------------------------------------------------------------------------------------
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and 16-byte aligned (a copy when it is not)."""
+def _dense(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``t`` in ``dtype``, contiguous and 16-byte aligned (a copy where it is not)."""
+    if dtype is not None and t.dtype != dtype:
+        t = t.to(dtype)
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -170,63 +172,76 @@ def _mx_addrs(buf: torch.Tensor, n: int, at: int = 0) -> Tuple[int, int]:
 def mxfp8_quantize(x: torch.Tensor) -> torch.Tensor:
     """MXFP8 copy of ``x`` (``fp_mxfp8_quantize``): a uint8 buffer of :func:`mxfp8_nbytes` bytes."""
     dev = require_cuda(x)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return mxfp8_quantize(x)
     dt = dtype_code(x.dtype)
     x = _dense(x)
     n = x.numel()
-    with _lib.on_device(dev):
-        buf = torch.empty(mxfp8_nbytes(n), dtype=torch.uint8, device=dev)
-        check(_lib.load().fp_mxfp8_quantize(x.data_ptr(), dt, n, *_mx_addrs(buf, n), _lib.raw_stream(dev)),
-              "fp_mxfp8_quantize")
+    buf = torch.empty(mxfp8_nbytes(n), dtype=torch.uint8, device=dev)
+    check(_lib.load().fp_mxfp8_quantize(x.data_ptr(), dt, n, *_mx_addrs(buf, n), _lib.raw_stream(dev)),
+          "fp_mxfp8_quantize")
     return buf
 
 
 def mxfp8_dequantize(buf: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
     """The values of an MXFP8 copy (``fp_mxfp8_dequantize``) in ``dtype`` and ``shape``."""
     dev = require_cuda(buf)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return mxfp8_dequantize(buf, shape, dtype)
     dt = dtype_code(dtype)
-    with _lib.on_device(dev):
-        y = torch.empty(shape, dtype=dtype, device=dev)
-        n = y.numel()
-        if buf.dtype != torch.uint8 or buf.numel() != mxfp8_nbytes(n):
-            raise ValueError(f"an MXFP8 copy of {n} elements is {mxfp8_nbytes(n)} uint8, got {buf.numel()} {buf.dtype}")
-        check(_lib.load().fp_mxfp8_dequantize(*_mx_addrs(_dense(buf), n), dt, n, y.data_ptr(), _lib.raw_stream(dev)),
-              "fp_mxfp8_dequantize")
+    n = torch.Size(shape).numel()
+    if buf.dtype != torch.uint8 or buf.numel() != mxfp8_nbytes(n):
+        raise ValueError(f"an MXFP8 copy of {n} elements is {mxfp8_nbytes(n)} uint8, got {buf.numel()} {buf.dtype}")
+    buf = _dense(buf)
+    y = torch.empty(shape, dtype=dtype, device=dev)
+    check(_lib.load().fp_mxfp8_dequantize(*_mx_addrs(buf, n), dt, n, y.data_ptr(), _lib.raw_stream(dev)),
+          "fp_mxfp8_dequantize")
     return y
+
+
+def _swiglu_half(n: int) -> int:
+    """Bytes from the copy of g to the copy of u in :func:`swiglu_fwd_mxfp8`'s buffer."""
+    return (mxfp8_nbytes(n) + 15) // 16 * 16
 
 
 def swiglu_fwd_mxfp8(g: torch.Tensor, u: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """h = silu(g) * u and the MXFP8 copies of g, then u, in one uint8 buffer (``fp_swiglu_fwd_mxfp8``)."""
     dev = require_cuda(g, u)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return swiglu_fwd_mxfp8(g, u)
     if g.shape != u.shape:
         raise ValueError(f"g and u must have the same shape, got {tuple(g.shape)} and {tuple(u.shape)}")
     dt = dtype_code(g.dtype)
-    g, u = _dense(g), _dense(u.to(g.dtype))
+    g, u = _dense(g), _dense(u, g.dtype)
     n = g.numel()
-    half = (mxfp8_nbytes(n) + 15) // 16 * 16
-    with _lib.on_device(dev):
-        h = torch.empty(g.shape, dtype=g.dtype, device=dev)
-        buf = torch.empty(2 * half, dtype=torch.uint8, device=dev)
-        check(_lib.load().fp_swiglu_fwd_mxfp8(g.data_ptr(), u.data_ptr(), dt, n, h.data_ptr(), *_mx_addrs(buf, n),
-                                              *_mx_addrs(buf, n, half), _lib.raw_stream(dev)), "fp_swiglu_fwd_mxfp8")
+    half = _swiglu_half(n)
+    h = torch.empty_like(g)
+    buf = torch.empty(2 * half, dtype=torch.uint8, device=dev)
+    check(_lib.load().fp_swiglu_fwd_mxfp8(g.data_ptr(), u.data_ptr(), dt, n, h.data_ptr(), *_mx_addrs(buf, n),
+                                          *_mx_addrs(buf, n, half), _lib.raw_stream(dev)), "fp_swiglu_fwd_mxfp8")
     return h, buf
 
 
 def swiglu_bwd_mxfp8(dout: torch.Tensor, buf: torch.Tensor, want_h: bool = False):
     """Backward of :func:`swiglu_fwd_mxfp8` (``fp_swiglu_bwd_mxfp8``): (dg, du, h or None), dout's dtype."""
     dev = require_cuda(dout, buf)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return swiglu_bwd_mxfp8(dout, buf, want_h)
     dt = dtype_code(dout.dtype)
-    dout = _dense(dout)
+    dout, buf = _dense(dout), _dense(buf)
     n = dout.numel()
-    half = (mxfp8_nbytes(n) + 15) // 16 * 16
+    half = _swiglu_half(n)
     if buf.dtype != torch.uint8 or buf.numel() != 2 * half:
         raise ValueError("the buffer is not that of swiglu_fwd_mxfp8 for as many elements")
-    buf = _dense(buf)
-    with _lib.on_device(dev):
-        dg, du = torch.empty_like(dout), torch.empty_like(dout)
-        h = torch.empty_like(dout) if want_h else None
-        check(_lib.load().fp_swiglu_bwd_mxfp8(dout.data_ptr(), *_mx_addrs(buf, n), *_mx_addrs(buf, n, half), dt, n,
-                                              dg.data_ptr(), du.data_ptr(), _addr(h), _lib.raw_stream(dev)),
-              "fp_swiglu_bwd_mxfp8")
+    dg, du = torch.empty_like(dout), torch.empty_like(dout)
+    h = torch.empty_like(dout) if want_h else None
+    check(_lib.load().fp_swiglu_bwd_mxfp8(dout.data_ptr(), *_mx_addrs(buf, n), *_mx_addrs(buf, n, half), dt, n,
+                                          dg.data_ptr(), du.data_ptr(), _addr(h), _lib.raw_stream(dev)),
+          "fp_swiglu_bwd_mxfp8")
     return dg, du, h
 
 
@@ -235,53 +250,67 @@ def router_scores_train(x: torch.Tensor, q_proj: torch.Tensor, block_keys: torch
     :func:`router_scores_bwd` needs of them, MXFP8 copy of x or None).  The second is one fp32 buffer: q16
     [M, 16], then rnorm [M]."""
     dev = require_cuda(x, q_proj, block_keys)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return router_scores_train(x, q_proj, block_keys, keep_mxfp8)
     dt = dtype_code(x.dtype)
-    x, q_proj, block_keys = _dense(x), _dense(q_proj.to(x.dtype)), _dense(block_keys.to(x.dtype))
+    x, q_proj, block_keys = _dense(x), _dense(q_proj, x.dtype), _dense(block_keys, x.dtype)
     D, NB = x.shape[-1], block_keys.shape[0]
     M = x.numel() // D
-    with _lib.on_device(dev):
-        scores = torch.empty(x.shape[:-1] + (NB,), dtype=torch.float32, device=dev)
-        saved = torch.empty(17 * M, dtype=torch.float32, device=dev)
-        buf = torch.empty(mxfp8_nbytes(M * D), dtype=torch.uint8, device=dev) if keep_mxfp8 else None
-        codes, scales = _mx_addrs(buf, M * D) if keep_mxfp8 and M > 0 else (None, None)
-        q16 = saved.data_ptr()
-        check(_lib.load().fp_router_scores_train(x.data_ptr(), q_proj.data_ptr(), block_keys.data_ptr(), dt, M, D, NB,
-                                                 scores.data_ptr(), q16, q16 + 64 * M, codes, scales,
-                                                 _lib.raw_stream(dev)), "fp_router_scores_train")
+    scores = torch.empty(x.shape[:-1] + (NB,), dtype=torch.float32, device=dev)
+    saved = torch.empty(17 * M, dtype=torch.float32, device=dev)
+    buf = torch.empty(mxfp8_nbytes(M * D), dtype=torch.uint8, device=dev) if keep_mxfp8 else None
+    codes, scales = _mx_addrs(buf, M * D) if keep_mxfp8 and M > 0 else (None, None)
+    q16 = saved.data_ptr()
+    check(_lib.load().fp_router_scores_train(x.data_ptr(), q_proj.data_ptr(), block_keys.data_ptr(), dt, M, D, NB,
+                                             scores.data_ptr(), q16, q16 + 64 * M, codes, scales,
+                                             _lib.raw_stream(dev)), "fp_router_scores_train")
     return scores, saved, buf
 
 
 def router_scores_bwd(dscores: torch.Tensor, x: Optional[torch.Tensor], buf: Optional[torch.Tensor],
                       q_proj: torch.Tensor, block_keys: torch.Tensor, saved: torch.Tensor, dtype: torch.dtype,
-                      grad_dtype: torch.dtype = torch.float32, want: Tuple[bool, bool, bool] = (True, True, True)):
-    """Gradient of the router scores (``fp_router_scores_bwd``): (dx [..., D], dq_proj, dblock_keys), None where
-    not ``want``ed.  dscores is [..., NB] fp32; the tokens come from ``x`` or, where given, from their MXFP8
-    copy ``buf``; ``dtype`` is theirs."""
+                      want: Tuple[bool, bool, bool] = (True, True, True)):
+    """Gradient of the router scores (``fp_router_scores_bwd``): (dx [..., D] in ``dtype``, dq_proj and
+    dblock_keys in their parameters' dtypes), None where not ``want``ed.  dscores is [..., NB]; the tokens come
+    from ``x`` or, where given, from their MXFP8 copy ``buf``; ``dtype`` is theirs."""
     dev = require_cuda(dscores, x, buf, q_proj, block_keys, saved)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return router_scores_bwd(dscores, x, buf, q_proj, block_keys, saved, dtype, want)
     dt = dtype_code(dtype)
-    dscores = _dense(dscores.float())
-    q_proj, block_keys = _dense(q_proj.to(dtype)), _dense(block_keys.to(dtype))
+    dscores = _dense(dscores, torch.float32)
+    w, k = _dense(q_proj, dtype), _dense(block_keys, dtype)
     x = _dense(x) if x is not None else None
-    NB, D = dscores.shape[-1], q_proj.shape[1]
+    NB, D = dscores.shape[-1], w.shape[1]
     M = dscores.numel() // NB
     if saved.numel() != 17 * M or (x is not None and x.numel() != M * D) or \
-            (buf is not None and buf.numel() != mxfp8_nbytes(M * D)) or block_keys.shape != (NB, 16):
+            (buf is not None and buf.numel() != mxfp8_nbytes(M * D)) or k.shape != (NB, 16):
         raise ValueError("the tensors are not those of router_scores_train for these shapes")
+    # both weight gradients leave in one dtype: the parameters' where they agree, else fp32
+    same = q_proj.dtype == block_keys.dtype
+    gd = q_proj.dtype if same else torch.float32
+    dx = dw = dk = None
+    if want[0]:
+        dx = torch.empty_like(x) if x is not None else torch.empty(dscores.shape[:-1] + (D,), dtype=dtype, device=dev)
+    if want[1]:
+        dw = torch.empty_like(w) if gd == dtype else torch.empty(16, D, dtype=gd, device=dev)
+    if want[2]:
+        dk = torch.empty_like(k) if gd == dtype else torch.empty(NB, 16, dtype=gd, device=dev)
+    if M == 0:
+        return (dx, torch.zeros_like(q_proj) if dw is not None else None,
+                torch.zeros_like(block_keys) if dk is not None else None)
     lib = _lib.load()
-    with _lib.on_device(dev):
-        dx = torch.empty(dscores.shape[:-1] + (D,), dtype=dtype, device=dev) if want[0] else None
-        dw = torch.empty(16, D, dtype=grad_dtype, device=dev) if want[1] else None
-        dk = torch.empty(NB, 16, dtype=grad_dtype, device=dev) if want[2] else None
-        if M == 0:
-            return dx, dw.zero_() if dw is not None else None, dk.zero_() if dk is not None else None
-        nbytes = lib.fp_router_scores_bwd_workspace_size(dt, M, D, NB)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        codes, scales = _mx_addrs(buf, M * D) if buf is not None else (None, None)
-        q16 = saved.data_ptr()
-        check(lib.fp_router_scores_bwd(dscores.data_ptr(), _addr(x), codes, scales, q_proj.data_ptr(),
-                                       block_keys.data_ptr(), q16, q16 + 64 * M, dt, M, D, NB, _addr(dx), _addr(dw),
-                                       _addr(dk), dtype_code(grad_dtype), ws.data_ptr(), nbytes,
-                                       _lib.raw_stream(dev)), "fp_router_scores_bwd")
+    nbytes = lib.fp_router_scores_bwd_workspace_size(dt, M, D, NB)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    codes, scales = _mx_addrs(buf, M * D) if buf is not None else (None, None)
+    q16 = saved.data_ptr()
+    check(lib.fp_router_scores_bwd(dscores.data_ptr(), _addr(x), codes, scales, w.data_ptr(), k.data_ptr(), q16,
+                                   q16 + 64 * M, dt, M, D, NB, _addr(dx), _addr(dw), _addr(dk), dtype_code(gd),
+                                   ws.data_ptr(), nbytes, _lib.raw_stream(dev)), "fp_router_scores_bwd")
+    if not same:
+        dw = dw.to(q_proj.dtype) if dw is not None else None
+        dk = dk.to(block_keys.dtype) if dk is not None else None
     return dx, dw, dk
 
 
@@ -290,11 +319,15 @@ def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[to
                      valid: Optional[torch.Tensor], counts_in: Optional[torch.Tensor] = None):
     """Counts of the routed blocks and, where ``scores`` [..., NB] fp32 are given, the balance loss
     (``fp_balance_loss_fwd``): (loss 0-d fp32 or None, counts [NB] int64, state [NB + 1] fp32 or None).
-    remote_indices [..., capacity] and remote_counts [...] int32, valid [...] bool."""
+    remote_indices [..., capacity] and remote_counts [...] integers, valid [...] bool."""
     dev = require_cuda(scores, remote_indices, remote_counts, valid, counts_in)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return balance_loss_fwd(scores, remote_indices, remote_counts, num_blocks, base_blocks, temperature, valid,
+                                    counts_in)
     scores = _dense(scores) if scores is not None else None
-    idx = _dense(remote_indices.to(torch.int32)) if remote_indices is not None else None
-    cnt = _dense(remote_counts.to(torch.int32)) if remote_counts is not None else None
+    idx = _dense(remote_indices, torch.int32) if remote_indices is not None else None
+    cnt = _dense(remote_counts, torch.int32) if remote_counts is not None else None
     valid = _dense(valid) if valid is not None else None
     counts_in = _dense(counts_in) if counts_in is not None else None
     M = scores.numel() // num_blocks if scores is not None else cnt.numel()
@@ -303,16 +336,15 @@ def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[to
         idx = cnt
     lib = _lib.load()
     loss = state = None
-    with _lib.on_device(dev):
-        counts = torch.empty(num_blocks, dtype=torch.int64, device=dev)
-        if scores is not None:
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            state = torch.empty(num_blocks + 1, dtype=torch.float32, device=dev)
-        nbytes = lib.fp_balance_workspace_size(M, num_blocks)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(lib.fp_balance_loss_fwd(_addr(scores), M, num_blocks, base_blocks, temperature, _addr(valid), _addr(idx),
-                                      _addr(cnt), cap, _addr(counts_in), counts.data_ptr(), _addr(loss), _addr(state),
-                                      ws.data_ptr(), nbytes, _lib.raw_stream(dev)), "fp_balance_loss_fwd")
+    counts = torch.empty(num_blocks, dtype=torch.int64, device=dev)
+    if scores is not None:
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        state = torch.empty(num_blocks + 1, dtype=torch.float32, device=dev)
+    nbytes = lib.fp_balance_workspace_size(M, num_blocks)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    check(lib.fp_balance_loss_fwd(_addr(scores), M, num_blocks, base_blocks, temperature, _addr(valid), _addr(idx),
+                                  _addr(cnt), cap, _addr(counts_in), counts.data_ptr(), _addr(loss), _addr(state),
+                                  ws.data_ptr(), nbytes, _lib.raw_stream(dev)), "fp_balance_loss_fwd")
     return loss, counts, state
 
 
@@ -320,15 +352,16 @@ def balance_loss_bwd(scores: torch.Tensor, base_blocks: int, temperature: float,
                      state: torch.Tensor, dloss: torch.Tensor) -> torch.Tensor:
     """dscores [..., NB] of :func:`balance_loss_fwd` (``fp_balance_loss_bwd``)."""
     dev = require_cuda(scores, valid, state, dloss)
+    if _lib.elsewhere(dev):
+        with torch.cuda.device(dev):
+            return balance_loss_bwd(scores, base_blocks, temperature, valid, state, dloss)
     scores = _dense(scores)
     valid = _dense(valid) if valid is not None else None
-    dloss = dloss.float()
     NB = scores.shape[-1]
-    with _lib.on_device(dev):
-        ds = torch.empty_like(scores)
-        check(_lib.load().fp_balance_loss_bwd(scores.data_ptr(), scores.numel() // NB, NB, base_blocks, temperature,
-                                              _addr(valid), state.data_ptr(), dloss.data_ptr(), ds.data_ptr(),
-                                              _lib.raw_stream(dev)), "fp_balance_loss_bwd")
+    ds = torch.empty_like(scores)
+    check(_lib.load().fp_balance_loss_bwd(scores.data_ptr(), scores.numel() // NB, NB, base_blocks, temperature,
+                                          _addr(valid), state.data_ptr(), dloss.data_ptr(), ds.data_ptr(),
+                                          _lib.raw_stream(dev)), "fp_balance_loss_bwd")
     return ds
 
 

@@ -28,11 +28,10 @@ from typing import Optional
 
 import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from . import kernels
 from ._lib import require_cuda
-from .training import check_checkpoint
+from .training import check_checkpoint, once
 
 ACTIVATIONS = tuple(kernels.PATTENTION_ACTIVATIONS)
 
@@ -63,11 +62,11 @@ class _SwiGLUCheckpoint(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dh):
         buf, = ctx.saved_tensors
         dg, du, _ = kernels.swiglu_bwd_mxfp8(dh, buf)
-        return dg, du.to(ctx.u_dtype)
+        return dg, du if du.dtype == ctx.u_dtype else du.to(ctx.u_dtype)
 
 
 def triton_fused_swiglu(g: Tensor, u: Tensor, *, checkpoint: Optional[str] = None) -> Tensor:
