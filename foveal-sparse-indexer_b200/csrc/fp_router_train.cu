@@ -1198,7 +1198,7 @@ balance_join_kernel(const float* __restrict__ psum, const int32_t* __restrict__ 
     state[NB] = n > 0 ? (float)((double)R / ((double)temperature * (double)n)) : 0.f;
   }
   if (grp == 0 && b < NB)
-    state[b] = total > 0 && remote ? (float)((double)(c * R - total) / ((double)total * R)) : 0.f;
+    state[b] = total > 0 && remote ? (float)(fma((double)c, (double)R, -(double)total) / ((double)total * R)) : 0.f;
 }
 
 template <int kE, bool kVec>

@@ -71,7 +71,7 @@ class _PooledTrain(torch.autograd.Function):
     @staticmethod
     def forward(ctx, module, x2d, k_gate, k_up, v, wq, k16, wout):
         packed = module._packed()
-        keep = module.checkpoint is not None
+        keep = check_checkpoint(module.checkpoint) is not None
         if keep:
             scores, saved, buf = kernels.router_scores_train(x2d, wq, k16, keep_mxfp8=True)
         else:
@@ -149,6 +149,8 @@ class _ForwardOnly(torch.autograd.Function):
 
 class FovealPattentionMLP(nn.Module):
     """Foveal block-sparse SwiGLU token-parameter attention (Pattention) layer."""
+
+    checkpoint: Optional[str] = None  # modules saved whole before this attribute existed
 
     def __init__(
         self,
@@ -334,10 +336,13 @@ class FovealPattentionMLP(nn.Module):
         scores = router_scores(xx, self.q_proj_16d.weight, self.block_keys_16d, checkpoint=self.checkpoint)
         s2d = scores.detach().reshape(-1, self.num_blocks)
         cap = max(int(self.max_remote_blocks), 1)
-        with torch.cuda.device(s2d.device):
-            idx, cnt, _, _ = kernels.select(s2d, base_blocks=self.base_blocks, top_p=self.top_p,
-                                            min_remote=self.min_remote_blocks, max_remote=self.max_remote_blocks,
-                                            capacity=cap, temperature=self.temperature)
+        if s2d.numel() == 0:  # no tokens: nothing to select from
+            idx, cnt = (torch.empty(n, dtype=torch.int32, device=s2d.device) for n in ((0, cap), (0,)))
+        else:
+            with torch.cuda.device(s2d.device):
+                idx, cnt, _, _ = kernels.select(s2d, base_blocks=self.base_blocks, top_p=self.top_p,
+                                                min_remote=self.min_remote_blocks, max_remote=self.max_remote_blocks,
+                                                capacity=cap, temperature=self.temperature)
         lead = x.shape[:-1]
         return balance_loss(scores, idx.view(*lead, cap), cnt.view(lead), base_blocks=self.base_blocks,
                             temperature=self.temperature, valid=valid)

@@ -295,6 +295,22 @@ def test_router_scores(M, D, NB, dtype, checkpoint):
     check_router(x, wq, k16, ds, checkpoint, (s, *grads))
 
 
+@pytest.mark.parametrize("D", [768, 2304, 4096, 8192])
+def test_router_scores_are_the_inference_scores(D):
+    """The training forward gives the same bits as fp_router_scores at wide inputs, and its 8-bit copy is
+    checkpoint_mxfp8's, NaN and infinities included."""
+    x, wq, k16, _ = router_case(75, D, 224, torch.bfloat16)
+    x[3, 5], x[4, D - 1], x[60, 33] = math.nan, math.inf, -3e38
+    ref = kernels.router_scores(x, wq, k16)[0]
+    for keep in (False, True):
+        s, _, buf = kernels.router_scores_train(x, wq, k16, keep_mxfp8=keep)
+        assert torch.equal(torch.nan_to_num(s, nan=7.0), torch.nan_to_num(ref, nan=7.0))
+        assert torch.equal(torch.isnan(s), torch.isnan(ref))
+    c = fsi.checkpoint_mxfp8(x)
+    n = x.numel()
+    assert torch.equal(buf[:n], c.buffer[:n]) and torch.equal(buf[-n // 32:], c.scales)
+
+
 def test_router_scores_partial_gradients():
     """Each subset of the inputs' gradients is that of all of them, bit by bit; leading dimensions, strides and
     weights of another type are taken."""
@@ -518,6 +534,8 @@ def test_balance_loss_given_counts():
     big = total * 10_000_000_000  # 64-bit counts
     loss, counts, ds = run_balance(s, None, None, 3, counts=big)
     assert torch.equal(counts, big) and abs(float(loss) - float(a[0])) <= 4 * U * float(a[0])
+    huge = total * 10 ** 15  # their products with the number of blocks pass 64 bits
+    check(run_balance(s, None, None, 3, counts=huge)[2], a[2], 8 * U * a[2].abs())
     check(ds, a[2], 8 * U * a[2].abs())
 
 
@@ -553,6 +571,86 @@ def test_balance_loss_against_differences():
     num = (f(s.double() + e * v) - f(s.double() - e * v)) / (2 * e)
     mag = float((ds.double() * v).abs().sum())
     assert abs(num - float((ds.double() * v).sum())) <= (100 * e * e + 256 * U) * mag
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+def test_checkpoint_past_32_bits():
+    n = 2 ** 31 + 4096 + 37
+    x = torch.empty(n, dtype=torch.bfloat16, device=DEV)
+    x[:1000] = 1.5
+    x[1000:-5000] = 0
+    tail = randn(5000 - 5000 % 32 + 37, seed=120, dtype=torch.bfloat16)  # from a block's border to the end
+    x[-tail.numel():] = tail
+    c = fsi.checkpoint_mxfp8(x)
+    y = c.restore()
+    assert torch.equal(y[-tail.numel():].double(), mx_ref(tail)[0])
+    assert bool((y[:1000] == 1.5).all()) and not bool(y[1000:-tail.numel()].any())
+    del x, y, c
+    torch.cuda.empty_cache()
+
+
+def test_swiglu_past_32_bits():
+    n = 2 ** 31 + 64
+    g = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    u = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    tg, tu, td = (randn(96, seed=s, dtype=torch.bfloat16) for s in (121, 122, 123))
+    g[-96:], u[-96:] = tg, tu
+    h, buf = kernels.swiglu_fwd_mxfp8(g, u)
+    ht, bt = kernels.swiglu_fwd_mxfp8(tg, tu)
+    assert torch.equal(h[-96:], ht) and not bool(h[:-96].any())
+    del h
+    g.zero_()
+    g[-96:] = td
+    dg, du, _ = kernels.swiglu_bwd_mxfp8(g, buf)
+    rg, ru, _ = kernels.swiglu_bwd_mxfp8(td, bt)
+    assert torch.equal(dg[-96:], rg) and torch.equal(du[-96:], ru) and not bool(dg[:-96].any())
+    del g, u, dg, du, buf
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+def test_router_past_32_bits(checkpoint):
+    """A row's scores and input gradient do not depend on the rows before it, and zero rows add nothing to the
+    weights' gradients."""
+    M, D, NB, last = 2 ** 19 + 70, 4096, 8, 70
+    x = torch.zeros(M, D, dtype=torch.bfloat16, device=DEV)
+    t, wq, k16, dt = router_case(last, D, NB, torch.bfloat16, seed=124)
+    x[-last:] = t
+    ds = torch.zeros(M, NB, device=DEV)
+    ds[-last:] = dt
+    s, saved, buf = kernels.router_scores_train(x, wq, k16, keep_mxfp8=checkpoint is not None)
+    st, saved_t, buf_t = kernels.router_scores_train(t, wq, k16, keep_mxfp8=checkpoint is not None)
+    assert torch.equal(s[-last:], st) and not bool(s[:-last].any())
+    a = kernels.router_scores_bwd(ds, None if buf is not None else x, buf, wq, k16, saved, torch.bfloat16)
+    b = kernels.router_scores_bwd(dt, None if buf is not None else t, buf_t, wq, k16, saved_t, torch.bfloat16)
+    assert torch.equal(a[0][-last:], b[0]) and not bool(a[0][:-last].any())
+    ref, mag, mag2 = router_ref(t, mx_ref(t)[0] if checkpoint else t, wq, k16, dt)
+    for i in (1, 2):
+        r = ref[i + 1]
+        check(a[i], r, half(torch.bfloat16) * r.abs() + (D + NB + last + 64) * U * mag[i + 1] + 2.0 ** -16 * mag2[i + 1])
+    del x, ds, s, saved, buf, a
+    torch.cuda.empty_cache()
+
+
+def test_balance_past_32_bits():
+    M, NB, last = 2 ** 21 + 21, 1024, 37
+    s = torch.zeros(M, NB, device=DEV)
+    t, idx, cnt = balance_case(last, NB, 4, 8, seed=125)
+    s[-last:] = t
+    ids = torch.zeros(M, 8, dtype=torch.int32, device=DEV)
+    ids[-last:] = idx
+    n = torch.zeros(M, dtype=torch.int32, device=DEV)
+    n[-last:] = cnt
+    valid = torch.zeros(M, dtype=torch.bool, device=DEV)
+    valid[-last:] = True
+    loss, counts, state = kernels.balance_loss_fwd(s, ids, n, NB, 4, 1.0, valid)
+    ref, rc, rds, tol, tl = balance_ref(t, idx, cnt, 4)
+    assert torch.equal(counts, rc) and abs(float(loss) - float(ref)) <= tl
+    ds = kernels.balance_loss_bwd(s, 4, 1.0, valid, state, torch.ones((), device=DEV))
+    check(ds[-last:], rds, tol + U * rds.abs() + 1e-37)
+    assert not bool(ds[:-last].any())
+    del s, ds, ids
+    torch.cuda.empty_cache()
 
 
 # ------------------------------------------------------------------ streams, graphs, determinism
@@ -623,6 +721,54 @@ def test_captured_and_replayed():
     graphs[1].replay()
     torch.cuda.synchronize()
     assert same(outs[0], step(*new)) and same(outs[1], ref[id(b)])
+
+
+def test_two_host_threads():
+    """Two threads with streams of their own give what each gives alone."""
+    import threading
+
+    ins = [step_inputs(60), step_inputs(70, M=333, D=520, NB=65)]
+    ref = [step(*i) for i in ins]
+    torch.cuda.synchronize()
+    ok = [True, True]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                out = step(*ins[k])
+                torch.cuda.current_stream().synchronize()
+                ok[k] = ok[k] and same(out, ref[k])
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(ok)
+
+
+def test_another_current_device(monkeypatch):
+    """Where another device is current, a call makes its tensors' device current first (each wrapper's own branch;
+    one GPU here, so the question is answered yes once per call)."""
+    ins = step_inputs(60)
+    ref = step(*ins)
+    seen = []
+
+    def once_elsewhere(device):
+        seen.append(device)
+        return len(seen) % 2 == 1
+
+    monkeypatch.setattr(fsi._lib, "elsewhere", once_elsewhere)
+    assert same(step(*ins), ref)
+    assert len(seen) == 2 * 8  # forward and backward of three operators, copy and restore
+
+
+def test_double_backward_refused():
+    x, wq, k16, ds = router_case(4, 64, 8, torch.float32)
+    x.requires_grad_()
+    g, = torch.autograd.grad(fsi.router_scores(x, wq, k16), x, ds, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
 
 
 # ------------------------------------------------------------------ the module
@@ -705,6 +851,21 @@ def test_module_balance_loss():
     assert rel_err(m.q_proj_16d.weight.grad, r[2]) <= 1e-4
     assert rel_err(m.block_keys_16d.grad, r[3]) <= 1e-4
     assert not bool(x.grad[1, 31:].any())
+
+
+def test_module_balance_loss_edges():
+    m = make_mlp(torch.bfloat16, "mxfp8")
+    loss, counts = m.balance_loss(torch.zeros(0, 256, dtype=torch.bfloat16, device=DEV))
+    assert float(loss.detach()) == 0.0 and not bool(counts.any())
+    loss, counts = m.balance_loss(randn(256, seed=115))  # one token, another type
+    assert loss.shape == () and int(counts.sum()) >= 1
+    m.checkpoint = "fp4"
+    with pytest.raises(ValueError):
+        m(randn(4, 256, seed=116, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        m.balance_loss(randn(4, 256, seed=116, dtype=torch.bfloat16))
+    del m.__dict__["checkpoint"]  # as in a module saved whole before the attribute existed
+    m(randn(4, 256, seed=116, dtype=torch.bfloat16)).sum().backward()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
