@@ -51,10 +51,10 @@ int device_info(int& num_sms);
 
 // ---- router.cu
 // k16f_cos (optional): fp32 block keys [NB, 16] of the cosine form (both sides L2-normalised,
-// compute_block_scores core.py:254-266) used instead of k16.  rnorm (optional): [M] factors 1 / rms(x Wq^T).
+// compute_block_scores core.py:254-266) used instead of k16.
 int launch_router_scores(const void* x, const void* wq, const void* k16, int dtype, int64_t M, int D,
                          int NB, float temperature, float* scores, float* q16, cudaStream_t st,
-                         const float* k16f_cos = nullptr, float* rnorm = nullptr);
+                         const float* k16f_cos = nullptr);
 struct SelectOut;
 int launch_select(const float* scores, int64_t M, int NB, int base, float top_p, int k_min, int k_max,
                   int capacity, float temperature, int32_t* idx, int32_t* cnt, const float* k16f,

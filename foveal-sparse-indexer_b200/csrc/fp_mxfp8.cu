@@ -10,11 +10,14 @@
 namespace fp {
 namespace {
 
-// All four kernels stream: a thread takes kUnroll vectors of 16 bytes, a CTA's width apart, and issues all of
-// their loads before the first use.  HBM bound.
+// All four kernels stream: a thread takes a few vectors of 16 bytes, a CTA's width apart, and issues all of their
+// loads before the first use.  HBM bound, but for the SwiGLU forward, which the exact division and exponential
+// of fp_swiglu_fwd (whose bits it keeps) hold at 0.92 of a copy's rate: with the hardware's approximations
+// it took 278 us where it takes 318 (16384 x 14336 bf16).  Vectors to a thread, measured there (GB/s moved;
+// torch's copy 6500): copy 4 / 8: 6470 / 6810; restore 2 / 4: 6680 / 6310; forward 1 / 2 / 4: 5470 / 5960 /
+// 5020; backward 1 / 2 / 4: 5970 / 5650 / 4800.  256 threads; 512 lost 5 to 15 %, 128 gained nothing sure.
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;      // one tensor in
-constexpr int kUnroll2 = 2;     // two or three tensors in
+constexpr int kUnrollCopy = 8, kUnrollRestore = 2, kUnrollFwd = 2, kUnrollBwd = 1;
 
 template <typename T, int U>
 __device__ __forceinline__ int64_t first_element() {
@@ -27,12 +30,12 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 mxfp8_quantize_kernel(const T* __restrict__ x, int64_t n, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   using V = MxVec<T>;
-  const int64_t i = first_element<T, kUnroll>();
-  uint4 w[kUnroll];
+  const int64_t i = first_element<T, kUnrollCopy>();
+  uint4 w[kUnrollCopy];
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) w[k] = V::load(x, i + k * kStep<T>, n);
+  for (int k = 0; k < kUnrollCopy; ++k) w[k] = V::load(x, i + k * kStep<T>, n);
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) V::quantize(w[k], i + k * kStep<T>, n, codes, scales);
+  for (int k = 0; k < kUnrollCopy; ++k) V::quantize(w[k], i + k * kStep<T>, n, codes, scales);
 }
 
 template <typename T>
@@ -40,12 +43,12 @@ __global__ void __launch_bounds__(kThreads)
 mxfp8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n,
                         T* __restrict__ y) {
   using V = MxVec<T>;
-  const int64_t i = first_element<T, kUnroll>();
-  typename V::Codes q[kUnroll];
+  const int64_t i = first_element<T, kUnrollRestore>();
+  typename V::Codes q[kUnrollRestore];
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) q[k] = V::load_codes(codes, scales, i + k * kStep<T>, n);
+  for (int k = 0; k < kUnrollRestore; ++k) q[k] = V::load_codes(codes, scales, i + k * kStep<T>, n);
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
+  for (int k = 0; k < kUnrollRestore; ++k) {
     float v[V::kV];
     V::values(q[k], v);
     V::store(y, i + k * kStep<T>, n, v);
@@ -58,15 +61,15 @@ swiglu_fwd_mxfp8_kernel(const T* __restrict__ g, const T* __restrict__ u, int64_
                         uint8_t* __restrict__ gc, uint8_t* __restrict__ gs, uint8_t* __restrict__ uc,
                         uint8_t* __restrict__ us) {
   using V = MxVec<T>;
-  const int64_t i0 = first_element<T, kUnroll2>();
-  uint4 gw[kUnroll2], uw[kUnroll2];
+  const int64_t i0 = first_element<T, kUnrollFwd>();
+  uint4 gw[kUnrollFwd], uw[kUnrollFwd];
 #pragma unroll
-  for (int k = 0; k < kUnroll2; ++k) {
+  for (int k = 0; k < kUnrollFwd; ++k) {
     gw[k] = V::load(g, i0 + k * kStep<T>, n);
     uw[k] = V::load(u, i0 + k * kStep<T>, n);
   }
 #pragma unroll
-  for (int k = 0; k < kUnroll2; ++k) {
+  for (int k = 0; k < kUnrollFwd; ++k) {
     const int64_t i = i0 + k * kStep<T>;
     V::quantize(gw[k], i, n, gc, gs);
     V::quantize(uw[k], i, n, uc, us);
@@ -96,17 +99,17 @@ swiglu_bwd_mxfp8_kernel(const T* __restrict__ dout, const uint8_t* __restrict__ 
                         const uint8_t* __restrict__ uc, const uint8_t* __restrict__ us, int64_t n,
                         T* __restrict__ dg, T* __restrict__ du, T* __restrict__ h) {
   using V = MxVec<T>;
-  const int64_t i0 = first_element<T, kUnroll2>();
-  uint4 dw[kUnroll2];
-  typename V::Codes gq[kUnroll2], uq[kUnroll2];
+  const int64_t i0 = first_element<T, kUnrollBwd>();
+  uint4 dw[kUnrollBwd];
+  typename V::Codes gq[kUnrollBwd], uq[kUnrollBwd];
 #pragma unroll
-  for (int k = 0; k < kUnroll2; ++k) {
+  for (int k = 0; k < kUnrollBwd; ++k) {
     dw[k] = V::load(dout, i0 + k * kStep<T>, n);
     gq[k] = V::load_codes(gc, gs, i0 + k * kStep<T>, n);
     uq[k] = V::load_codes(uc, us, i0 + k * kStep<T>, n);
   }
 #pragma unroll
-  for (int k = 0; k < kUnroll2; ++k) {
+  for (int k = 0; k < kUnrollBwd; ++k) {
     const int64_t i = i0 + k * kStep<T>;
     float d[V::kV], gv[V::kV], uv[V::kV];
     V::unpack(dw[k], d);
@@ -162,7 +165,7 @@ int fp_mxfp8_quantize(const void* x, int dtype, int64_t n, void* codes, void* sc
   if (!x || !codes || !scales || !al16(x) || !al16(codes)) return FP_ERR_INVALID_ARG;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned grid = grid_for<T>(n, kUnroll);
+    const unsigned grid = grid_for<T>(n, kUnrollCopy);
     if (!grid) return FP_ERR_UNSUPPORTED;
     mxfp8_quantize_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T*)x, n, (uint8_t*)codes,
                                                                          (uint8_t*)scales);
@@ -177,7 +180,7 @@ int fp_mxfp8_dequantize(const void* codes, const void* scales, int dtype, int64_
   if (!y || !codes || !scales || !al16(y) || !al16(codes)) return FP_ERR_INVALID_ARG;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned grid = grid_for<T>(n, kUnroll);
+    const unsigned grid = grid_for<T>(n, kUnrollRestore);
     if (!grid) return FP_ERR_UNSUPPORTED;
     mxfp8_dequantize_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const uint8_t*)codes,
                                                                            (const uint8_t*)scales, n, (T*)y);
@@ -194,7 +197,7 @@ int fp_swiglu_fwd_mxfp8(const void* g, const void* u, int dtype, int64_t n, void
   if (!al16(g) || !al16(u) || !al16(h) || !al16(g_codes) || !al16(u_codes)) return FP_ERR_INVALID_ARG;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned grid = grid_for<T>(n, kUnroll2);
+    const unsigned grid = grid_for<T>(n, kUnrollFwd);
     if (!grid) return FP_ERR_UNSUPPORTED;
     swiglu_fwd_mxfp8_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>(
         (const T*)g, (const T*)u, n, (T*)h, (uint8_t*)g_codes, (uint8_t*)g_scales, (uint8_t*)u_codes,
@@ -212,7 +215,7 @@ int fp_swiglu_bwd_mxfp8(const void* dout, const void* g_codes, const void* g_sca
   if (!al16(dout) || !al16(dg) || !al16(du) || !al16(h) || !al16(g_codes) || !al16(u_codes)) return FP_ERR_INVALID_ARG;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned grid = grid_for<T>(n, kUnroll2);
+    const unsigned grid = grid_for<T>(n, kUnrollBwd);
     if (!grid) return FP_ERR_UNSUPPORTED;
     swiglu_bwd_mxfp8_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>(
         (const T*)dout, (const uint8_t*)g_codes, (const uint8_t*)g_scales, (const uint8_t*)u_codes,

@@ -47,8 +47,7 @@ template <typename T>
 __global__ void __launch_bounds__(kScoreWarps * 32)
 router_scores_kernel(const T* __restrict__ x, const T* __restrict__ wq, const T* __restrict__ k16,
                      int64_t M, int D, int NB, float inv_scale_div, float temperature,
-                     float* __restrict__ scores, float* __restrict__ q16_out, const float* __restrict__ kcos,
-                     float* __restrict__ rnorm_out) {
+                     float* __restrict__ scores, float* __restrict__ q16_out, const float* __restrict__ kcos) {
   extern __shared__ float sk[];  // [16][NB] fp32 block keys, transposed: lanes read consecutive blocks
   if (kcos) {
     // cosine form: keys L2-normalised in fp32 (F.normalize: k / max(||k||, 1e-12))
@@ -124,7 +123,6 @@ router_scores_kernel(const T* __restrict__ x, const T* __restrict__ wq, const T*
       for (int j = 1; j < 16; ++j) qv = (lane == j) ? q[j] : qv;
       q16_out[tok * 16 + lane] = qv;
     }
-    if (rnorm_out && lane == 0) rnorm_out[tok] = inv;
     if (kcos) {  // normalize(rms_norm(q)) of compute_block_scores
       float qq = 0.f;
 #pragma unroll
@@ -174,8 +172,7 @@ __device__ __forceinline__ void ld32B(const __nv_bfloat16* p, uint32_t (&w)[8]) 
 __global__ void __launch_bounds__(kMmaWarps * 32)
 router_scores_mma_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ wq,
                          const __nv_bfloat16* __restrict__ k16, int64_t M, int D, int NB,
-                         float* __restrict__ scores, float* __restrict__ q16_out, const float* __restrict__ kcos,
-                         float* __restrict__ rnorm_out) {
+                         float* __restrict__ scores, float* __restrict__ q16_out, const float* __restrict__ kcos) {
   extern __shared__ float sk[];  // [16][NB] transposed block keys, then [kMmaWarps][16][17] partials
   float* sq = sk + 16 * NB;
   if (kcos) {
@@ -250,7 +247,6 @@ router_scores_mma_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat1
       qv[j] *= inv;
     }
     if (q16_out && lane < 16) q16_out[tok * 16 + lane] = qown * inv;
-    if (rnorm_out && lane == 0) rnorm_out[tok] = inv;
     if (kcos) {  // normalize(rms_norm(q)) of compute_block_scores
       float qq = 0.f;
 #pragma unroll
@@ -1188,7 +1184,7 @@ pooled_topk_kernel(const float* __restrict__ mean_vec, const T* __restrict__ wq,
 // ============================================================================================
 int launch_router_scores(const void* x, const void* wq, const void* k16, int dtype, int64_t M, int D,
                          int NB, float temperature, float* scores, float* q16, cudaStream_t st,
-                         const float* kcos, float* rnorm) {
+                         const float* kcos) {
   if (M <= 0) return FP_OK;
   if (dtype == FP_DTYPE_BF16 && D % (64 * kMmaWarps) == 0 && temperature == 1.0f) {
     const size_t smem = (size_t)NB * 16 * sizeof(float) + kMmaWarps * 16 * 17 * sizeof(float);
@@ -1198,8 +1194,7 @@ int launch_router_scores(const void* x, const void* wq, const void* k16, int dty
       return FP_ERR_CUDA;
     const int blocks = (int)((M + 15) / 16);
     router_scores_mma_kernel<<<blocks, kMmaWarps * 32, smem, st>>>(
-        (const __nv_bfloat16*)x, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)k16, M, D, NB, scores, q16, kcos,
-        rnorm);
+        (const __nv_bfloat16*)x, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)k16, M, D, NB, scores, q16, kcos);
     return cudaGetLastError() == cudaSuccess ? FP_OK : FP_ERR_CUDA;
   }
   const int blocks = (int)((M + kScoreWarps * kScoreTPW - 1) / (kScoreWarps * kScoreTPW));
@@ -1213,10 +1208,10 @@ int launch_router_scores(const void* x, const void* wq, const void* k16, int dty
   if (dtype == FP_DTYPE_BF16)
     router_scores_kernel<__nv_bfloat16><<<blocks, kScoreWarps * 32, smem, st>>>(
         (const __nv_bfloat16*)x, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)k16, M, D, NB, 0.25f,
-        temperature, scores, q16, kcos, rnorm);
+        temperature, scores, q16, kcos);
   else
     router_scores_kernel<float><<<blocks, kScoreWarps * 32, smem, st>>>(
-        (const float*)x, (const float*)wq, (const float*)k16, M, D, NB, 0.25f, temperature, scores, q16, kcos, rnorm);
+        (const float*)x, (const float*)wq, (const float*)k16, M, D, NB, 0.25f, temperature, scores, q16, kcos);
   return cudaGetLastError() == cudaSuccess ? FP_OK : FP_ERR_CUDA;
 }
 

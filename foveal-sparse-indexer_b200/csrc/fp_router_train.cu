@@ -91,9 +91,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // stays for many tiles of 32 tokens, with the block keys in shared memory once (loaded per 16 tokens they took
 // as long as the projection), a key serves four tokens from registers, and the normalisation factor and
 // (kKeep) the MXFP8 copy of x leave in the same pass over x.  Warp: one quarter of D, 16 tokens; then 4
-// tokens' scores.  HBM bound by x.
+// tokens' scores.  HBM bound by x (16384 x 4096: 36 us, 4.1 TB/s; with the copy 55 us, 4.0 TB/s).
+// With the copy, x comes by TMA (64 columns x 16 tokens) into a ring that a warp keeps for itself and that runs
+// on through the scores of a tile (55 us; loads into registers 59 us: the quantisation leaves too few in
+// flight).  Without it, plain loads of two steps at a time do better (36 us; the ring 42 us: W_q's fragments
+// come through L1, which the ring shrinks).
 constexpr int kFwWarps = 8;
 constexpr int kFwTokens = 32;
+constexpr int kFwStages = 4;
+constexpr int kFwRing = kFwWarps * kFwStages * 2048;
 
 // MXFP8 codes of 16 consecutive bf16 values (w: in order); the lane's neighbour (lane ^ 1) holds the other half of
 // the block.  All lanes of the warp call this together.
@@ -131,51 +137,119 @@ __device__ __forceinline__ void load32(const __nv_bfloat16* p, uint32_t (&w)[8])
   w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
 }
 
+// 32 bytes as two pieces of shared memory.
+__device__ __forceinline__ void lds32(const uint8_t* p, const uint8_t* q, uint32_t (&w)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p), v = *reinterpret_cast<const uint4*>(q);
+  w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w; w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
+}
+
 template <bool kKeep>
 __global__ void __launch_bounds__(kFwWarps * 32, 2)
-router_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ wq,
-                  const __nv_bfloat16* __restrict__ k16, int64_t M, int D, int NB, float* __restrict__ scores,
+router_fwd_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __restrict__ x,
+                  const __nv_bfloat16* __restrict__ wq, const __nv_bfloat16* __restrict__ k16, int64_t M, int D, int NB, float* __restrict__ scores,
                   float* __restrict__ q16, float* __restrict__ rnorm, uint8_t* __restrict__ codes,
                   uint8_t* __restrict__ scales) {
-  extern __shared__ float skeys[];               // [16][NB] block keys
+  extern __shared__ uint8_t fw_dyn[];
+  uint8_t* ring = fw_dyn + (1024 - (smem_u32(fw_dyn) & 1023)) % 1024;  // [warp][stage] tiles of x
+  float* skeys = reinterpret_cast<float*>(ring + (kKeep ? kFwRing : 0));  // [16][NB] block keys
+  __shared__ uint64_t bars[kFwWarps][kFwStages];
   __shared__ float sq[2][4][16 * 17];            // [token group][quarter of D] partial projections
   __shared__ float4 sv[kFwTokens * 4];           // [token][16] projections
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int quarter = warp & 3, group = warp >> 2, dpart = D / 4, kbeg = quarter * dpart;
+  const int tiles = (int)((M + kFwTokens - 1) / kFwTokens);
+  uint8_t* xs = ring + warp * kFwStages * 2048;
+  int f_tile = blockIdx.x, f_k = 0, f_stage = 0;  // the next copy (lane 0)
+  const auto fetch = [&] {
+    if (f_tile >= tiles) return;
+    mbar_arrive_expect_tx(&bars[warp][f_stage], 2048);
+    tma_load_2d(xs + f_stage * 2048, &map, &bars[warp][f_stage], kbeg + f_k, f_tile * kFwTokens + 16 * group);
+    f_stage = (f_stage + 1) % kFwStages;
+    f_k += 64;
+    if (f_k == dpart) {
+      f_k = 0;
+      f_tile += gridDim.x;
+    }
+  };
+  if (kKeep && lane == 0) {
+    for (int k = 0; k < kFwStages; ++k) mbar_init(&bars[warp][k], 1);
+    fence_mbar_init();
+    for (int k = 0; k < kFwStages; ++k) fetch();
+  }
   for (int i = threadIdx.x; i < NB * kIdx; i += blockDim.x) {
     const int j = i / NB, b = i - j * NB;
     skeys[i] = __bfloat162float(k16[b * kIdx + j]);
   }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int quarter = warp & 3, group = warp >> 2, dpart = D / 4, kbeg = quarter * dpart;
+  __syncthreads();  // keys and barriers
   const __nv_bfloat16* wa = wq + (int64_t)g * D + kbeg + 16 * t;
   const __nv_bfloat16* wb = wa + (int64_t)8 * D;
-  for (int64_t tok0 = (int64_t)blockIdx.x * kFwTokens; tok0 < M; tok0 += (int64_t)gridDim.x * kFwTokens) {
+  int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  uint32_t B0[8], B1[8];  // kKeep: W_q's fragments of the step to come
+  if constexpr (kKeep) {
+    load32(wa, B0);
+    load32(wb, B1);
+  }
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t tok0 = (int64_t)tile * kFwTokens;
     const int64_t ta = tok0 + 16 * group + g, tb = ta + 8;
-    const int64_t oa = (ta < M ? ta : M - 1) * D + kbeg + 16 * t, ob = (tb < M ? tb : M - 1) * D + kbeg + 16 * t;
     float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (int k0 = 0; k0 < dpart; k0 += 64) {
-      uint32_t A0[8], A1[8], B0[8], B1[8];
-      load32(x + oa + k0, A0);
-      load32(x + ob + k0, A1);
-      load32(wa + k0, B0);
-      load32(wb + k0, B1);
+    if constexpr (kKeep) {
+#pragma unroll 1
+      for (int k0 = 0; k0 < dpart && ok; k0 += 64) {
+        uint32_t A0[8], A1[8];
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], parity, nullptr, 0));
+        if (!ok) break;
+        // 128-byte swizzle: 16-byte piece ^ row % 8; rows g and g + 8, pieces 2 t and 2 t + 1
+        const uint8_t* r = xs + stage * 2048 + g * 128;
+        const int p0 = ((2 * t) ^ g) << 4, p1 = ((2 * t + 1) ^ g) << 4;
+        lds32(r + p0, r + p1, A0);
+        lds32(r + 1024 + p0, r + 1024 + p1, A1);
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        mma_bf16(c0, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], B0[2 * st], B0[2 * st + 1]);
-        mma_bf16(c1, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], B1[2 * st], B1[2 * st + 1]);
-      }
-      if constexpr (kKeep) {
+        for (int st = 0; st < 4; ++st) {
+          mma_bf16(c0, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], B0[2 * st], B0[2 * st + 1]);
+          mma_bf16(c1, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], B1[2 * st], B1[2 * st + 1]);
+        }
+        const int kn = k0 + 64 < dpart ? k0 + 64 : 0;
+        load32(wa + kn, B0);
+        load32(wb + kn, B1);
+        __syncwarp();  // the tile is in every lane's registers
+        if (lane == 0) fetch();
+        if (++stage == kFwStages) {
+          stage = 0;
+          parity ^= 1;
+        }
+        const int64_t col = kbeg + k0 + 16 * t;
         uint4 q;
         int byte;
         mx_quantize16(A0, q, byte);
         if (ta < M) {
-          *reinterpret_cast<uint4*>(codes + oa + k0) = q;
-          if (!(t & 1)) scales[(oa + k0) / kMxBlock] = (uint8_t)byte;
+          *reinterpret_cast<uint4*>(codes + ta * D + col) = q;
+          if (!(t & 1)) scales[(ta * D + col) / kMxBlock] = (uint8_t)byte;
         }
         mx_quantize16(A1, q, byte);
         if (tb < M) {
-          *reinterpret_cast<uint4*>(codes + ob + k0) = q;
-          if (!(t & 1)) scales[(ob + k0) / kMxBlock] = (uint8_t)byte;
+          *reinterpret_cast<uint4*>(codes + tb * D + col) = q;
+          if (!(t & 1)) scales[(tb * D + col) / kMxBlock] = (uint8_t)byte;
+        }
+      }
+      if (!ok)  // a copy did not arrive within the wait limit: the tile's scores become NaN, and all that follow
+        c0[0] = c0[1] = c0[2] = c0[3] = __uint_as_float(0x7FC00000u);
+    } else {
+      const __nv_bfloat16* xa = x + (ta < M ? ta : M - 1) * D + kbeg + 16 * t;
+      const __nv_bfloat16* xb = x + (tb < M ? tb : M - 1) * D + kbeg + 16 * t;
+#pragma unroll 2
+      for (int k0 = 0; k0 < dpart; k0 += 64) {
+        uint32_t A0[8], A1[8], W0[8], W1[8];
+        load32(xa + k0, A0);
+        load32(xb + k0, A1);
+        load32(wa + k0, W0);
+        load32(wb + k0, W1);
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          mma_bf16(c0, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], W0[2 * st], W0[2 * st + 1]);
+          mma_bf16(c1, A0[2 * st], A1[2 * st], A0[2 * st + 1], A1[2 * st + 1], W1[2 * st], W1[2 * st + 1]);
         }
       }
     }
@@ -236,17 +310,173 @@ router_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __re
     }
     __syncthreads();  // the partial projections' place is free again
   }
+  if (!ok)  // copies under way end before their place does
+    for (int k = 1; k < kFwStages; ++k) {
+      if (++stage == kFwStages) {
+        stage = 0;
+        parity ^= 1;
+      }
+      mbar_wait(&bars[warp][stage], parity, nullptr, 0);
+    }
+}
+
+// The same for fp32 and for widths that are not a multiple of 256: fp_router_scores' CUDA-core kernel in its
+// order of sums (lane: columns 8 lane + 256 i, then a butterfly), so the same bits.  What held that kernel at
+// 270 us (16384 x 4096 fp32) were W_q's loads, 16 rows of them one after the other for each step of x; here a
+// step's W_q (256 columns) is in shared memory, copied one step ahead for the CTA's 32 tokens, and x is loaded
+// one step ahead.  Bound by the FMA units and shared memory (512 and 136 wavefronts a step) for fp32.
+constexpr int kAnyTokens = 4;  // of a warp
+
+template <typename T>
+struct Raw8 {  // 8 consecutive elements
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void unpack(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      const uint4 a = w[0], b = w[1];
+      v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+      v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+    } else {
+      const uint32_t r[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(r[i] << 16);
+        v[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kFwWarps * 32, 1)
+router_fwd_any_kernel(const T* __restrict__ x, const T* __restrict__ wq, const T* __restrict__ k16, int64_t M, int D,
+                      int NB, float* __restrict__ scores, float* __restrict__ q16, float* __restrict__ rnorm) {
+  constexpr int kPieces = sizeof(T) / 2;                // 16-byte pieces of 8 elements
+  constexpr int kStep = 16 * kPieces * 32;              // of one step of W_q
+  extern __shared__ uint4 any_dyn[];                    // [2][16][piece][lane] W_q, then [16][NB] block keys
+  float* skeys = reinterpret_cast<float*>(any_dyn + 2 * kStep);
+  for (int i = threadIdx.x; i < NB * kIdx; i += blockDim.x) {
+    const int j = i / NB, b = i - j * NB;
+    skeys[i] = to_f32(k16[b * kIdx + j]);
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int steps = (D + 255) / 256;
+  const auto copy_w = [&](int step) {
+    if (step < steps) {
+      for (int i = threadIdx.x; i < kStep; i += kFwWarps * 32) {
+        const int l = (i / kPieces) & 31, j = i / (kPieces * 32), piece = i % kPieces;  // along a row of W_q
+        const int c = step * 256 + l * 8;
+        if (c < D)
+          cp_async_16(smem_u32(any_dyn + (step & 1) * kStep + (j * kPieces + piece) * 32 + l),
+                      reinterpret_cast<const uint4*>(wq + (int64_t)j * D + c) + piece);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int64_t base = (int64_t)blockIdx.x * (kFwWarps * kAnyTokens); base < M; base += (int64_t)gridDim.x * (kFwWarps * kAnyTokens)) {
+    const int64_t tok0 = base + warp * kAnyTokens;
+    const int live = (int)max((int64_t)0, min((int64_t)kAnyTokens, M - tok0));
+    float acc[kAnyTokens][kIdx];
+    Raw8<T> next[kAnyTokens];
+#pragma unroll
+    for (int r = 0; r < kAnyTokens; ++r)
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) acc[r][j] = 0.f;
+    const auto load_x = [&](int step) {
+      const int c = step * 256 + lane * 8;
+#pragma unroll
+      for (int r = 0; r < kAnyTokens; ++r)
+        if (c < D) next[r].load(x + (tok0 + r < M ? tok0 + r : M - 1) * D + c);
+    };
+    __syncthreads();  // keys; W_q's first place is free
+    copy_w(0);
+    load_x(0);
+    for (int step = 0; step < steps; ++step) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();
+      copy_w(step + 1);
+      float xv[kAnyTokens][8];
+#pragma unroll
+      for (int r = 0; r < kAnyTokens; ++r) next[r].unpack(xv[r]);
+      if (step + 1 < steps) load_x(step + 1);
+      if (step * 256 + lane * 8 < D) {
+        const uint4* w = any_dyn + (step & 1) * kStep + lane;
+#pragma unroll
+        for (int j = 0; j < kIdx; ++j) {
+          Raw8<T> raw;
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) raw.w[i] = w[(j * kPieces + i) * 32];
+          float wv[8];
+          raw.unpack(wv);
+#pragma unroll
+          for (int r = 0; r < kAnyTokens; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r][j] = fmaf(xv[r][e], wv[e], acc[r][j]);
+        }
+      }
+    }
+    const float eps = 1.1920928955078125e-07f;  // torch.finfo(float32).eps: F.rms_norm's default
+#pragma unroll
+    for (int r = 0; r < kAnyTokens; ++r) {
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) acc[r][j] = warp_sum(acc[r][j]);
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) ss = fmaf(acc[r][j], acc[r][j], ss);
+      const float inv = __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / 16.0f) + eps));
+      float own = 0.f;
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) {
+        acc[r][j] *= inv;
+        if (lane == j) own = acc[r][j];
+      }
+      if (r < live) {
+        if (lane < kIdx) q16[(tok0 + r) * kIdx + lane] = own;
+        if (lane == 0) rnorm[tok0 + r] = inv;
+      }
+    }
+    for (int b = lane; b < NB; b += 32) {
+      float sc[kAnyTokens] = {};
+#pragma unroll
+      for (int j = 0; j < kIdx; ++j) {
+        const float kv = skeys[j * NB + b];
+#pragma unroll
+        for (int r = 0; r < kAnyTokens; ++r) sc[r] = fmaf(acc[r][j], kv, sc[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < kAnyTokens; ++r)
+        if (r < live) scores[(tok0 + r) * NB + b] = sc[r] * 0.25f;  // / sqrt(16)
+    }
+  }
+}
+
+template <typename T>
+int launch_router_fwd_any(const void* x, const void* wq, const void* k16, int64_t M, int D, int NB, float* scores,
+                          float* q16, float* rnorm, int sms, cudaStream_t st) {
+  constexpr auto kern = router_fwd_any_kernel<T>;
+  constexpr int ring = 2 * 16 * 256 * (int)sizeof(T);
+  if (!allow_smem<kern>(ring + 64 * 1024)) return FP_ERR_CUDA;
+  const int64_t tiles = (M + kFwWarps * kAnyTokens - 1) / (kFwWarps * kAnyTokens);
+  kern<<<(int)std::min<int64_t>(tiles, 2 * sms), kFwWarps * 32, ring + NB * kIdx * 4, st>>>(
+      (const T*)x, (const T*)wq, (const T*)k16, M, D, NB, scores, q16, rnorm);
+  return launched();
 }
 
 template <bool kKeep>
 int launch_router_fwd(const void* x, const void* wq, const void* k16, int64_t M, int D, int NB, float* scores,
                       float* q16, float* rnorm, void* codes, void* scales, int sms, cudaStream_t st) {
   constexpr auto kern = router_fwd_kernel<kKeep>;
-  const size_t smem = (size_t)NB * kIdx * 4;  // at most 64 KB
-  if (smem > 36 * 1024 && !allow_smem<kern>(64 * 1024)) return FP_ERR_CUDA;
+  constexpr int ring = kKeep ? kFwRing : 0;
+  const int smem = 1024 + ring + NB * kIdx * 4;  // at most 129 KB
+  if (!allow_smem<kern>(1024 + ring + 64 * 1024)) return FP_ERR_CUDA;
+  CUtensorMap map{};
+  if (kKeep && !encode_map_2d(&map, x, D, M, (uint64_t)D * 2, 64, 16)) return FP_ERR_CUDA;
   const int grid = (int)std::min<int64_t>((M + kFwTokens - 1) / kFwTokens, 2 * sms);
-  kern<<<grid, kFwWarps * 32, smem, st>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)k16,
-                                          M, D, NB, scores, q16, rnorm, (uint8_t*)codes, (uint8_t*)scales);
+  kern<<<grid, kFwWarps * 32, smem, st>>>(map, (const __nv_bfloat16*)x, (const __nv_bfloat16*)wq,
+                                          (const __nv_bfloat16*)k16, M, D, NB, scores, q16, rnorm, (uint8_t*)codes, (uint8_t*)scales);
   return launched();
 }
 
@@ -538,7 +768,7 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
   int stage = 0, tile = tile0;
   uint32_t parity = 0;
   for (; tile < tiles; tile += hop) {
-    if (!mbar_wait(bars + stage, parity, nullptr, 0)) break;
+    if (!__all_sync(0xffffffffu, mbar_wait(bars + stage, parity, nullptr, 0))) break;
     const uint4* q = reinterpret_cast<const uint4*>(qs + stage * 1024);
     const uint4 h4 = q[lane], l4 = q[32 + lane];
     uint4 r[4];
@@ -647,13 +877,15 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
   }
 }
 
-// Pass 2, fp32, on the FMA units (32 per element): a thread owns 4 columns (their Wq and dWq in registers),
-// dq of 32 tokens at a time in shared memory; tx threads (32, 64, 128) lie along the columns, 128 / tx along
-// tokens.  x runs through a ring of kFAhead tokens that a thread keeps for itself (cp.async; with two loads
-// in flight from registers the pass took 238 us at 16384 x 4096).
+// Pass 2, fp32, on the FMA units (32 per element): a thread owns 4 columns (their Wq and dWq in registers), dq (and
+// the copy's scales) of 32 tokens at a time in shared memory; tx threads (32, 64, 128) lie along the columns,
+// 128 / tx along tokens.  x runs through a ring of kFAhead tokens that a thread keeps for itself (cp.async).
+// Issue bound: 16384 x 4096 took 238 us with two loads in flight from registers, 166 us with the ring (3.2
+// TB/s); paired FMAs (fma.rn.f32x2) need fewer instructions, spill, and took 175 to 194 us.
 constexpr int kFThreads = 128;
 constexpr int kFTokens = 32;
 constexpr int kFAhead = 8;
+constexpr int kFScales = kFThreads * 4 / kMxBlock + 1;  // blocks that a CTA's columns of a token may touch
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -667,11 +899,12 @@ __global__ void __launch_bounds__(kFThreads, 3)
 router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                     const float* __restrict__ dq, const float* __restrict__ wq, int64_t M, int D, int tx,
                     int64_t tokens_per_cta, float* __restrict__ dx, float* __restrict__ dw_part) {
-  __shared__ float4 sq[kFTokens * 4];
-  __shared__ float red[kFThreads * 4 * kIdx];  // during the pass its first half is the ring [kFAhead][thread] float4
+  __shared__ float4 sq[kFTokens * 4];           // [token][16] dq
+  __shared__ uint8_t ss[kCodes ? kFTokens * kFScales : 1];  // [token][block] scale bytes
+  __shared__ float red[kFThreads * 4 * kIdx];   // during the pass its first half is the ring [kFAhead][thread] float4
   griddep_launch_dependents();
   const int lane = threadIdx.x % tx, ty = threadIdx.x / tx, nty = kFThreads / tx;
-  const int d = (blockIdx.x * tx + lane) * 4;
+  const int db = blockIdx.x * tx * 4, d = db + lane * 4, width = tx * 4;
   const bool in = d < D;
   float w[kIdx][4], acc[kIdx][4];
 #pragma unroll
@@ -695,17 +928,18 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
 #pragma unroll
   for (int k = 0; k < kFAhead - 1; ++k) fetch(first + (int64_t)k * nty, k);
   int slot = 0;
-  uint32_t byte = 127u;
-  const auto fetch_scale = [&](int64_t tok) {
-    if constexpr (kCodes)
-      if (in && dw_part && tok < t1) byte = __ldg(scales + (tok * D + d) / kMxBlock);
-  };
-  fetch_scale(first);
   griddep_wait();
   for (int64_t t0 = (int64_t)blockIdx.y * tokens_per_cta; t0 < t1; t0 += kFTokens) {
     const int n = (int)min((int64_t)kFTokens, t1 - t0);
     __syncthreads();
     for (int i = threadIdx.x; i < n * 4; i += kFThreads) sq[i] = __ldg(reinterpret_cast<const float4*>(dq + t0 * kIdx) + i);
+    if constexpr (kCodes) {
+      if (dw_part)
+        for (int i = threadIdx.x; i < n * kFScales; i += kFThreads) {
+          const int64_t row = (t0 + i / kFScales) * D, b = (row + db) / kMxBlock + i % kFScales;
+          if (b * kMxBlock < row + min(D, db + width)) ss[i] = __ldg(scales + b);
+        }
+    }
     __syncthreads();
     if (!in) continue;
 #pragma unroll 2
@@ -719,8 +953,7 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
       if (dw_part) {
         if constexpr (kCodes) {
           const uint32_t c = *reinterpret_cast<const uint32_t*>(mine);
-          const float s = mx_scale((int)byte);
-          fetch_scale(t0 + k + nty);
+          const float s = mx_scale((int)ss[k * kFScales + (int)(i / kMxBlock - (i - lane * 4) / kMxBlock)]);
           const float2 a = mx_unpack2((uint16_t)c), b = mx_unpack2((uint16_t)(c >> 16));
           v[0] = a.x * s; v[1] = a.y * s; v[2] = b.x * s; v[3] = b.y * s;
         } else {
@@ -746,7 +979,6 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
   }
   cp_async_wait<0>();
   if (!dw_part) return;
-  const int width = tx * 4;
   __syncthreads();  // the ring's place takes the sums
 #pragma unroll
   for (int j = 0; j < kIdx; ++j)
@@ -754,7 +986,6 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
     for (int e = 0; e < 4; ++e) red[(ty * kIdx + j) * width + lane * 4 + e] = acc[j][e];
   __syncthreads();
   float* part = dw_part + (int64_t)blockIdx.y * kIdx * D;
-  const int db = blockIdx.x * width;
   for (int i = threadIdx.x; i < kIdx * width; i += kFThreads) {
     const int j = i / width, c = i % width;
     float s = 0.f;
@@ -1342,7 +1573,9 @@ int fp_router_scores_train(const void* x, const void* q_proj, const void* block_
   if (dtype == FP_DTYPE_BF16 && D % 256 == 0)
     return codes ? launch_router_fwd<true>(x, q_proj, block_keys, M, D, NB, scores, q16, rnorm, codes, scales, sms, st)
                  : launch_router_fwd<false>(x, q_proj, block_keys, M, D, NB, scores, q16, rnorm, codes, scales, sms, st);
-  if (const int rc = launch_router_scores(x, q_proj, block_keys, dtype, M, D, NB, 1.0f, scores, q16, st, nullptr, rnorm))
+  if (const int rc = dtype == FP_DTYPE_BF16
+                         ? launch_router_fwd_any<__nv_bfloat16>(x, q_proj, block_keys, M, D, NB, scores, q16, rnorm, sms, st)
+                         : launch_router_fwd_any<float>(x, q_proj, block_keys, M, D, NB, scores, q16, rnorm, sms, st))
     return rc;
   return codes ? fp_mxfp8_quantize(x, dtype, M * D, codes, scales, stream) : FP_OK;
 }
