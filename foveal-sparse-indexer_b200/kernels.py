@@ -155,6 +155,11 @@ def _dense(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _empty(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    # sizes one by one: a tuple takes half as long again to parse, a torch.Size twice as long
+    return torch.empty(*shape, dtype=dtype, device=device) if len(shape) else torch.empty((), dtype=dtype, device=device)
+
+
 def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -195,7 +200,7 @@ def mxfp8_dequantize(buf: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tens
     if buf.dtype != torch.uint8 or buf.numel() != mxfp8_nbytes(n):
         raise ValueError(f"an MXFP8 copy of {n} elements is {mxfp8_nbytes(n)} uint8, got {buf.numel()} {buf.dtype}")
     buf = _dense(buf)
-    y = torch.empty(shape, dtype=dtype, device=dev)
+    y = _empty(shape, dtype, dev)
     check(_lib.load().fp_mxfp8_dequantize(*_mx_addrs(buf, n), dt, n, y.data_ptr(), _lib.raw_stream(dev)),
           "fp_mxfp8_dequantize")
     return y
@@ -257,7 +262,7 @@ def router_scores_train(x: torch.Tensor, q_proj: torch.Tensor, block_keys: torch
     x, q_proj, block_keys = _dense(x), _dense(q_proj, x.dtype), _dense(block_keys, x.dtype)
     D, NB = x.shape[-1], block_keys.shape[0]
     M = x.numel() // D
-    scores = torch.empty(x.shape[:-1] + (NB,), dtype=torch.float32, device=dev)
+    scores = _empty((*x.shape[:-1], NB), torch.float32, dev)
     saved = torch.empty(17 * M, dtype=torch.float32, device=dev)
     buf = torch.empty(mxfp8_nbytes(M * D), dtype=torch.uint8, device=dev) if keep_mxfp8 else None
     codes, scales = _mx_addrs(buf, M * D) if keep_mxfp8 and M > 0 else (None, None)
@@ -292,7 +297,7 @@ def router_scores_bwd(dscores: torch.Tensor, x: Optional[torch.Tensor], buf: Opt
     gd = q_proj.dtype if same else torch.float32
     dx = dw = dk = None
     if want[0]:
-        dx = torch.empty_like(x) if x is not None else torch.empty(dscores.shape[:-1] + (D,), dtype=dtype, device=dev)
+        dx = torch.empty_like(x) if x is not None else _empty((*dscores.shape[:-1], D), dtype, dev)
     if want[1]:
         dw = torch.empty_like(w) if gd == dtype else torch.empty(16, D, dtype=gd, device=dev)
     if want[2]:
@@ -314,6 +319,11 @@ def router_scores_bwd(dscores: torch.Tensor, x: Optional[torch.Tensor], buf: Opt
     return dx, dw, dk
 
 
+def _as_int32(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as int32; values past its range stay past every valid id and count (they do not wrap)."""
+    return t if t.dtype == torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
 def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[torch.Tensor],
                      remote_counts: Optional[torch.Tensor], num_blocks: int, base_blocks: int, temperature: float,
                      valid: Optional[torch.Tensor], counts_in: Optional[torch.Tensor] = None):
@@ -326,8 +336,8 @@ def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[to
             return balance_loss_fwd(scores, remote_indices, remote_counts, num_blocks, base_blocks, temperature, valid,
                                     counts_in)
     scores = _dense(scores) if scores is not None else None
-    idx = _dense(remote_indices, torch.int32) if remote_indices is not None else None
-    cnt = _dense(remote_counts, torch.int32) if remote_counts is not None else None
+    idx = _dense(_as_int32(remote_indices)) if remote_indices is not None else None
+    cnt = _dense(_as_int32(remote_counts)) if remote_counts is not None else None
     valid = _dense(valid) if valid is not None else None
     counts_in = _dense(counts_in) if counts_in is not None else None
     M = scores.numel() // num_blocks if scores is not None else cnt.numel()

@@ -508,6 +508,9 @@ def test_balance_loss_route_lists():
     check_balance(s, ids, cnt, 3)
     a, b = run_balance(s, idx, cnt, 3), run_balance(s, idx.long(), cnt.long(), 3)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+    far, n = idx.long(), cnt.long()  # 64-bit values that would wrap into range
+    far[0, 0], far[1, 0], n[2] = 2 ** 32 + 5, -2 ** 32 + 5, 2 ** 32
+    check_balance(s, far, n, 3)
 
 
 def test_balance_loss_even_load_and_collapse():

@@ -46,6 +46,19 @@ def test_unknown_checkpoint():
             call()
 
 
+def test_checkpoint_argument_reaches_the_module():
+    dense = torch.nn.Module()
+    for name, a, b in (("gate_proj", 64, 256), ("up_proj", 64, 256), ("down_proj", 256, 64)):
+        setattr(dense, name, torch.nn.Linear(a, b, bias=False))
+    layer = torch.nn.Module()
+    layer.mlp = dense
+    model = torch.nn.Module()
+    model.layers = torch.nn.ModuleList([layer])
+    fsi.sparsify_model_with_foveal_pattention(model, base_blocks=1, remote_blocks=2, checkpoint="mxfp8")
+    assert model.layers[0].mlp.checkpoint == "mxfp8"
+    assert fsi.FovealPattentionMLP(64, 128, base_blocks=1, remote_blocks=1).checkpoint is None
+
+
 @pytest.mark.parametrize("x,wq,k", [((4, 60), (16, 60), (8, 16)), ((4, 64), (8, 64), (8, 16)), ((4, 64), (16, 32), (8, 16)),
                                     ((4, 64), (16, 64), (8, 8)), ((4, 64), (16, 64), (1025, 16)),
                                     ((4, 64), (16, 64), (0, 16)), ((4, 0), (16, 0), (8, 16)), ((), (16, 1), (8, 16))])
