@@ -14,10 +14,12 @@ namespace {
 // loads before the first use.  HBM bound, but for the SwiGLU forward, which the exact division and exponential
 // of fp_swiglu_fwd (whose bits it keeps) hold at 0.92 of a copy's rate: with the hardware's approximations
 // it took 278 us where it takes 318 (16384 x 14336 bf16).  Vectors to a thread, measured there (GB/s moved;
-// torch's copy 6500): copy 4 / 8: 6470 / 6810; restore 2 / 4: 6680 / 6310; forward 1 / 2 / 4: 5470 / 5960 /
+// torch's copy 6500): copy 4 / 8: 6470 / 6810 (fp32, 16384 x 4096: 47 / 52 us); restore 2 / 4: 6680 / 6310; forward 1 / 2 / 4: 5470 / 5960 /
 // 5020; backward 1 / 2 / 4: 5970 / 5650 / 4800.  256 threads; 512 lost 5 to 15 %, 128 gained nothing sure.
 constexpr int kThreads = 256;
-constexpr int kUnrollCopy = 8, kUnrollRestore = 2, kUnrollFwd = 2, kUnrollBwd = 1;
+template <typename T>
+constexpr int kUnrollCopy = sizeof(T) == 2 ? 8 : 4;
+constexpr int kUnrollRestore = 2, kUnrollFwd = 2, kUnrollBwd = 1;
 
 template <typename T, int U>
 __device__ __forceinline__ int64_t first_element() {
@@ -30,12 +32,12 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 mxfp8_quantize_kernel(const T* __restrict__ x, int64_t n, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   using V = MxVec<T>;
-  const int64_t i = first_element<T, kUnrollCopy>();
-  uint4 w[kUnrollCopy];
+  const int64_t i = first_element<T, kUnrollCopy<T>>();
+  uint4 w[kUnrollCopy<T>];
 #pragma unroll
-  for (int k = 0; k < kUnrollCopy; ++k) w[k] = V::load(x, i + k * kStep<T>, n);
+  for (int k = 0; k < kUnrollCopy<T>; ++k) w[k] = V::load(x, i + k * kStep<T>, n);
 #pragma unroll
-  for (int k = 0; k < kUnrollCopy; ++k) V::quantize(w[k], i + k * kStep<T>, n, codes, scales);
+  for (int k = 0; k < kUnrollCopy<T>; ++k) V::quantize(w[k], i + k * kStep<T>, n, codes, scales);
 }
 
 template <typename T>
@@ -165,7 +167,7 @@ int fp_mxfp8_quantize(const void* x, int dtype, int64_t n, void* codes, void* sc
   if (!x || !codes || !scales || !al16(x) || !al16(codes)) return FP_ERR_INVALID_ARG;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned grid = grid_for<T>(n, kUnrollCopy);
+    const unsigned grid = grid_for<T>(n, kUnrollCopy<T>);
     if (!grid) return FP_ERR_UNSUPPORTED;
     mxfp8_quantize_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T*)x, n, (uint8_t*)codes,
                                                                          (uint8_t*)scales);

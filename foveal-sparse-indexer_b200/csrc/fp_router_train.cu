@@ -510,25 +510,42 @@ __device__ __forceinline__ void load_row16(const __nv_bfloat16* p, float (&v)[16
   }
 }
 
-// Four columns of one row of dS, zeros outside.
-__device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, int64_t M, int b, int NB, bool vec) {
-  if (t >= M || b >= NB) return make_float4(0.f, 0.f, 0.f, 0.f);
-  const float* p = ds + t * NB + b;
-  if (vec) return __ldg(reinterpret_cast<const float4*>(p));
-  return make_float4(p[0], b + 1 < NB ? p[1] : 0.f, b + 2 < NB ? p[2] : 0.f, b + 3 < NB ? p[3] : 0.f);
+// Four columns of one row of dS, zeros outside.  The loads are unconditional, from a place inside the tensor, so
+// that a loop's loads can be issued together (behind a branch they went one by one: 22 us for dq at
+// 16384 x 448).  kVec: NB % 4 == 0.
+template <bool kVec>
+__device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, int64_t M, int b, int NB) {
+  const bool in = t < M;
+  const float* row = ds + (in ? t : M - 1) * NB;
+  float4 v;
+  if constexpr (kVec) {
+    v = __ldg(reinterpret_cast<const float4*>(row + min(b, NB - 4)));
+    if (!in || b >= NB) v = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    v.x = __ldg(row + min(b, NB - 1));
+    v.y = __ldg(row + min(b + 1, NB - 1));
+    v.z = __ldg(row + min(b + 2, NB - 1));
+    v.w = __ldg(row + min(b + 3, NB - 1));
+    if (!in || b >= NB) v.x = 0.f;
+    if (!in || b + 1 >= NB) v.y = 0.f;
+    if (!in || b + 2 >= NB) v.z = 0.f;
+    if (!in || b + 3 >= NB) v.w = 0.f;
+  }
+  return v;
 }
 
 constexpr int kDqWarps = 8;
 constexpr int kDqTokens = 8 * kDqWarps;  // tokens of a CTA's tile
 constexpr int kDqMaxCtas = 296;
 
-// Pass 1.  Phase A, 8 tokens to a warp: a^T[j, tok] = K^T[j, b] dS^T[b, tok], then dq.  Phase B, a share of
-// the blocks (kG groups of 32) to a warp, over the CTA's 64 tokens (rows just read, from L1): dK^T[j, b] =
+// Pass 1.  CTAs of two kinds, running side by side (one after the other in each CTA they took 31 us at 16384 x 448).
+// dq (blockIdx.y = 0 where dq is wanted): 8 tokens to a warp, a^T[j, tok] = K^T[j, b] dS^T[b, tok], then dq.
+// dK (the other rows of the grid, 256 blocks each): 32 blocks to a warp over the CTA's 64 tokens, dK^T[j, b] =
 // n^T[j, tok] dS[tok, b], kept in registers over all of the CTA's tiles.  The order of b within a product and
 // the columns of a tile are permuted so that a lane's elements are 16 contiguous bytes.
 // dq: kPacked, per tile of 16 tokens the two bf16 pieces as pass 2's fragments ([tile][hi, lo][lane] uint4);
 // otherwise fp32 [M, 16].
-template <typename T, int kG, bool kPacked>
+template <typename T, bool kPacked, bool kVec>
 __global__ void __launch_bounds__(kDqWarps * 32)
 router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const float* __restrict__ q16,
                  const float* __restrict__ rnorm, int64_t M, int NB, void* __restrict__ dq_out,
@@ -537,8 +554,8 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int nk = (NB + 15) / 16;
-  const bool vec = (NB & 3) == 0;
-  if (dq_out) {
+  const bool for_dq = dq_out && blockIdx.y == 0;
+  if (for_dq) {
     // the first tile's rows start towards L2 while K goes to shared memory, one row of K to a thread
     const int64_t row0 = (int64_t)blockIdx.x * kDqTokens + 8 * warp;
     const int64_t bytes = min((int64_t)8, M - row0) * NB * 4;
@@ -556,18 +573,18 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
     }
     __syncthreads();
   }
-  float dk[kG][4][4];
+  // dK: the warp's blocks b0 + 0..31
+  const int b0 = 32 * (kDqWarps * ((int)blockIdx.y - (dq_out ? 1 : 0)) + warp);
+  float dk[4][4];
 #pragma unroll
-  for (int i = 0; i < kG; ++i)
+  for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dk[i][k][e] = 0.f;
+    for (int e = 0; e < 4; ++e) dk[k][e] = 0.f;
 
   for (int64_t base = (int64_t)blockIdx.x * kDqTokens; base < M; base += (int64_t)gridDim.x * kDqTokens) {
     const int64_t tok0 = base + 8 * warp;
     // (a tile of 16 tokens that ends past M is written whole: zeros behind the last token)
-    if (dq_out && tok0 < (M + 15) / 16 * 16) {
+    if (for_dq && tok0 < (M + 15) / 16 * 16) {
       float c[4] = {}, cl[4] = {};
       float n0[2], n1[2], r[2];  // of tokens 2 t and 2 t + 1
 #pragma unroll
@@ -582,7 +599,7 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
       }
 #pragma unroll 8
       for (int k = 0; k < nk; ++k) {
-        const float4 v = ds4(ds, tok0 + g, M, 16 * k + 4 * t, NB, vec);
+        const float4 v = ds4<kVec>(ds, tok0 + g, M, 16 * k + 4 * t, NB);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const float4 kv = sk[(k * 2 + s) * 32 + lane];
@@ -635,45 +652,42 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
         o[64] = make_uint2(lo[0], lo[1]);
       }
     }
-    if (dk_part) {
+    if (!for_dq && b0 < NB) {
       const int64_t end = min(base + kDqTokens, M);
-#pragma unroll (kG == 1 ? 4 : kG == 2 ? 2 : 1)
+#pragma unroll 4
       for (int64_t s0 = base; s0 < end; s0 += 8) {
         const int64_t ta = s0 + t, tb = s0 + t + 4;
         uint32_t nh[4], nl[4];
-        const float n4[4] = {ta < M ? q16[ta * kIdx + g] : 0.f, ta < M ? q16[ta * kIdx + g + 8] : 0.f,
-                             tb < M ? q16[tb * kIdx + g] : 0.f, tb < M ? q16[tb * kIdx + g + 8] : 0.f};
+        // (past the last token dS is zero, and the row read in its place is a token's)
+        const float* qa = q16 + min(ta, M - 1) * kIdx + g;
+        const float* qb = q16 + min(tb, M - 1) * kIdx + g;
+        const bool ia = ta < M, ib = tb < M;
+        const float n4[4] = {ia ? __ldg(qa) : 0.f, ia ? __ldg(qa + 8) : 0.f, ib ? __ldg(qb) : 0.f, ib ? __ldg(qb + 8) : 0.f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) tf32_split(n4[e], nh[e], nl[e]);
+        const float4 va = ds4<kVec>(ds, ta, M, b0 + 4 * g, NB), vb = ds4<kVec>(ds, tb, M, b0 + 4 * g, NB);
+        const float fa[4] = {va.x, va.y, va.z, va.w}, fb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
-        for (int i = 0; i < kG; ++i) {
-          const int b = 32 * (warp + kDqWarps * i) + 4 * g;
-          const float4 va = ds4(ds, ta, M, b, NB, vec), vb = ds4(ds, tb, M, b, NB, vec);
-          const float fa[4] = {va.x, va.y, va.z, va.w}, fb[4] = {vb.x, vb.y, vb.z, vb.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t h0, l0, h1, l1;
-            tf32_split(fa[k], h0, l0);
-            tf32_split(fb[k], h1, l1);
-            mma_tf32(dk[i][k], nh, l0, l1);
-            mma_tf32(dk[i][k], nl, h0, h1);
-            mma_tf32(dk[i][k], nh, h0, h1);
-          }
+        for (int k = 0; k < 4; ++k) {
+          uint32_t h0, l0, h1, l1;
+          tf32_split(fa[k], h0, l0);
+          tf32_split(fb[k], h1, l1);
+          mma_tf32(dk[k], nh, l0, l1);
+          mma_tf32(dk[k], nl, h0, h1);
+          mma_tf32(dk[k], nh, h0, h1);
         }
       }
     }
   }
-  if (dk_part) {  // dk[i][k]: b = 32 (..) + 8 t + k (+4: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
+  if (!for_dq) {  // dk[k]: b = b0 + 8 t + k (+4: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
     float* o = dk_part + (int64_t)blockIdx.x * NB * kIdx;
 #pragma unroll
-    for (int i = 0; i < kG; ++i)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int b = 32 * (warp + kDqWarps * i) + 8 * t + 4 * (e & 1) + k;
-          if (b < NB) o[b * kIdx + g + 8 * (e >> 1)] = dk[i][k][e] * 0.25f;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int b = b0 + 8 * t + 4 * (e & 1) + k;
+        if (b < NB) o[b * kIdx + g + 8 * (e >> 1)] = dk[k][e] * 0.25f;
+      }
   }
 }
 
@@ -1055,13 +1069,15 @@ BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
   return p;
 }
 
-template <typename T, int kG>
+template <typename T, bool kVec>
 int launch_dq(const BwdPlan& p, const float* ds, const T* k16, const float* q16, const float* rnorm, int64_t M, int NB,
               void* dq, float* pk, cudaStream_t st) {
-  constexpr auto kern = router_dq_kernel<T, kG, sizeof(T) == 2>;
+  constexpr auto kern = router_dq_kernel<T, sizeof(T) == 2, kVec>;
   const size_t smem = dq ? (size_t)((NB + 15) / 16) * 1024 : 0;  // at most 64 KB
   if (smem > 48 * 1024 && !allow_smem<kern>(64 * 1024)) return FP_ERR_CUDA;
-  kern<<<p.dq_ctas, kDqWarps * 32, smem, st>>>(ds, k16, q16, rnorm, M, NB, dq, pk);
+  const int rows = (dq ? 1 : 0) + (pk ? (NB + 32 * kDqWarps - 1) / (32 * kDqWarps) : 0);
+  if (rows == 0) return FP_OK;
+  kern<<<dim3(p.dq_ctas, rows), kDqWarps * 32, smem, st>>>(ds, k16, q16, rnorm, M, NB, dq, pk);
   return launched();
 }
 
@@ -1073,11 +1089,9 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
   void* dq = dx || dwq ? ws + p.dq : nullptr;
   float* pw = dwq ? reinterpret_cast<float*>(ws + p.dw) : nullptr;
   float* pk = dk16 ? reinterpret_cast<float*>(ws + p.dk) : nullptr;
-  int rc;
-  if (NB <= 256) rc = launch_dq<T, 1>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
-  else if (NB <= 512) rc = launch_dq<T, 2>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
-  else rc = launch_dq<T, 4>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st);
-  if (rc) return rc;
+  if (const int rc = NB % 4 == 0 ? launch_dq<T, true>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st)
+                                 : launch_dq<T, false>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st))
+    return rc;
   if (dq) {
     const dim3 grid(p.col_ctas, p.parts);
     cudaError_t e;
