@@ -328,7 +328,7 @@ def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[to
                      remote_counts: Optional[torch.Tensor], num_blocks: int, base_blocks: int, temperature: float,
                      valid: Optional[torch.Tensor], counts_in: Optional[torch.Tensor] = None):
     """Counts of the routed blocks and, where ``scores`` [..., NB] fp32 are given, the balance loss
-    (``fp_balance_loss_fwd``): (loss 0-d fp32 or None, counts [NB] int64, state [NB + 1] fp32 or None).
+    (``fp_balance_loss_fwd``): (loss 0-d fp32 or None, counts [NB] int64, state for the gradient or None).
     remote_indices [..., capacity] and remote_counts [...] integers, valid [...] bool."""
     dev = require_cuda(scores, remote_indices, remote_counts, valid, counts_in)
     if _lib.elsewhere(dev):
@@ -347,14 +347,16 @@ def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[to
     lib = _lib.load()
     loss = state = None
     counts = torch.empty(num_blocks, dtype=torch.int64, device=dev)
-    if scores is not None:
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        state = torch.empty(num_blocks + 1, dtype=torch.float32, device=dev)
+    # the state and the workspace are one buffer: at most 270 KB, kept until the backward pass
+    at = (num_blocks * 4 + 4 + 15) // 16 * 16
     nbytes = lib.fp_balance_workspace_size(M, num_blocks)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    buf = torch.empty(at + nbytes, dtype=torch.uint8, device=dev)
+    ws = buf.data_ptr() + at
+    if scores is not None:
+        loss, state = torch.empty((), dtype=torch.float32, device=dev), buf
     check(lib.fp_balance_loss_fwd(_addr(scores), M, num_blocks, base_blocks, temperature, _addr(valid), _addr(idx),
                                   _addr(cnt), cap, _addr(counts_in), counts.data_ptr(), _addr(loss), _addr(state),
-                                  ws.data_ptr(), nbytes, _lib.raw_stream(dev)), "fp_balance_loss_fwd")
+                                  ws, nbytes, _lib.raw_stream(dev)), "fp_balance_loss_fwd")
     return loss, counts, state
 
 

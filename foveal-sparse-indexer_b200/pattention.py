@@ -73,10 +73,9 @@ def triton_fused_swiglu(g: Tensor, u: Tensor, *, checkpoint: Optional[str] = Non
     """SwiGLU of two pre-activation tensors (pattention_triton.py:98-104), differentiable.  With
     ``checkpoint="mxfp8"`` the backward pass reads 8-bit copies of g and u (same h; half of bf16's bytes
     are held between the passes) and the gradients are those at the copies' values."""
-    check_checkpoint(checkpoint)
-    require_cuda(g, u)
-    if checkpoint is not None and torch.is_grad_enabled() and (g.requires_grad or u.requires_grad):
+    if checkpoint is not None and check_checkpoint(checkpoint) and torch.is_grad_enabled() and (g.requires_grad or u.requires_grad):
         return _SwiGLUCheckpoint.apply(g, u)
+    require_cuda(g, u)
     return TritonFusedSwiGLUFunction.apply(g, u)
 
 

@@ -22,7 +22,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import kernels
-from ._lib import dtype_code, require_cuda
+from ._lib import dtype_code
 
 CHECKPOINTS = (None, "mxfp8")
 
@@ -111,7 +111,6 @@ def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: 
     NB = block_keys.shape[0]
     if D == 0 or D % 8 or not 1 <= NB <= 1024:
         raise ValueError(f"the router takes widths that are multiples of 8 and 1 to 1024 blocks, got D {D}, NB {NB}")
-    require_cuda(x, q_proj, block_keys)
     grad = torch.is_grad_enabled() and (x.requires_grad or q_proj.requires_grad or block_keys.requires_grad)
     return _RouterScores.apply(x, q_proj, block_keys, grad and checkpoint is not None)
 
@@ -199,7 +198,6 @@ def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts
         if remote_counts.shape != lead:
             raise ValueError(f"routes of {tuple(remote_counts.shape)} rows for scores of {tuple(lead)}")
     _check_valid(valid, lead)
-    require_cuda(scores, remote_indices, remote_counts, valid, counts)
     if scores.dtype != torch.float32:
         scores = scores.float()
     return _BalanceLoss.apply(scores, remote_indices, remote_counts, int(base_blocks), float(temperature), valid, counts)
