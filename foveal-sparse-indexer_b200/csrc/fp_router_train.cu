@@ -20,6 +20,7 @@ namespace fp {
 namespace {
 
 constexpr int kIdx = 16;  // the router's width
+constexpr int kMaxWidth = 1 << 24;
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 int launched() { return cudaGetLastError() == cudaSuccess ? FP_OK : FP_ERR_CUDA; }
@@ -146,9 +147,9 @@ __device__ __forceinline__ void lds32(const uint8_t* p, const uint8_t* q, uint32
 template <bool kKeep>
 __global__ void __launch_bounds__(kFwWarps * 32, 2)
 router_fwd_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* __restrict__ x,
-                  const __nv_bfloat16* __restrict__ wq, const __nv_bfloat16* __restrict__ k16, int64_t M, int D, int NB, float* __restrict__ scores,
-                  float* __restrict__ q16, float* __restrict__ rnorm, uint8_t* __restrict__ codes,
-                  uint8_t* __restrict__ scales) {
+                  const __nv_bfloat16* __restrict__ wq, const __nv_bfloat16* __restrict__ k16, int64_t M, int D,
+                  int NB, float* __restrict__ scores, float* __restrict__ q16, float* __restrict__ rnorm,
+                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   extern __shared__ uint8_t fw_dyn[];
   uint8_t* ring = fw_dyn + (1024 - (smem_u32(fw_dyn) & 1023)) % 1024;  // [warp][stage] tiles of x
   float* skeys = reinterpret_cast<float*>(ring + (kKeep ? kFwRing : 0));  // [16][NB] block keys
@@ -310,13 +311,13 @@ router_fwd_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* 
     }
     __syncthreads();  // the partial projections' place is free again
   }
-  if (!ok)  // copies under way end before their place does
-    for (int k = 1; k < kFwStages; ++k) {
+  if (!ok)  // once more for the copies under way, before their place goes
+    for (int k = 0; k < kFwStages; ++k) {
+      mbar_wait(&bars[warp][stage], parity, nullptr, 0);
       if (++stage == kFwStages) {
         stage = 0;
         parity ^= 1;
       }
-      mbar_wait(&bars[warp][stage], parity, nullptr, 0);
     }
 }
 
@@ -376,7 +377,8 @@ router_fwd_any_kernel(const T* __restrict__ x, const T* __restrict__ wq, const T
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  for (int64_t base = (int64_t)blockIdx.x * (kFwWarps * kAnyTokens); base < M; base += (int64_t)gridDim.x * (kFwWarps * kAnyTokens)) {
+  constexpr int kTile = kFwWarps * kAnyTokens;
+  for (int64_t base = (int64_t)blockIdx.x * kTile; base < M; base += (int64_t)gridDim.x * kTile) {
     const int64_t tok0 = base + warp * kAnyTokens;
     const int live = (int)max((int64_t)0, min((int64_t)kAnyTokens, M - tok0));
     float acc[kAnyTokens][kIdx];
@@ -476,7 +478,8 @@ int launch_router_fwd(const void* x, const void* wq, const void* k16, int64_t M,
   if (kKeep && !encode_map_2d(&map, x, D, M, (uint64_t)D * 2, 64, 16)) return FP_ERR_CUDA;
   const int grid = (int)std::min<int64_t>((M + kFwTokens - 1) / kFwTokens, 2 * sms);
   kern<<<grid, kFwWarps * 32, smem, st>>>(map, (const __nv_bfloat16*)x, (const __nv_bfloat16*)wq,
-                                          (const __nv_bfloat16*)k16, M, D, NB, scores, q16, rnorm, (uint8_t*)codes, (uint8_t*)scales);
+                                          (const __nv_bfloat16*)k16, M, D, NB, scores, q16, rnorm, (uint8_t*)codes,
+                                          (uint8_t*)scales);
   return launched();
 }
 
@@ -488,7 +491,7 @@ int launch_router_fwd(const void* x, const void* wq, const void* k16, int64_t M,
 //
 // Precision.  Pass 1 multiplies fp32 values as tf32 pieces, v = hi + lo (the rest is below 2^-22 of v):
 // hi hi + hi lo + lo hi, fp32 accumulators.  Pass 2 with bf16 x holds dq as two bf16 pieces (rest below
-// 2^-17 of dq, against 2^-9 for the bf16 gradients), x and Wq are exact.  fp32 x stays on the FMA units.
+// 2^-17 of dq, against 2^-8 for the bf16 gradients), x and Wq are exact.  fp32 x stays on the FMA units.
 //
 // Fragment coordinates below: lane = 4 g + t, g = 0..7, t = 0..3.
 
@@ -550,7 +553,7 @@ __global__ void __launch_bounds__(kDqWarps * 32)
 router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const float* __restrict__ q16,
                  const float* __restrict__ rnorm, int64_t M, int NB, void* __restrict__ dq_out,
                  float* __restrict__ dk_part) {
-  extern __shared__ float4 sk[];  // [ceil(NB / 16)][2][32]: K as phase A's fragments
+  extern __shared__ float4 sk[];  // [ceil(NB / 16)][2][32]: K as the dq products' fragments
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int nk = (NB + 15) / 16;
@@ -662,7 +665,8 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
         const float* qa = q16 + min(ta, M - 1) * kIdx + g;
         const float* qb = q16 + min(tb, M - 1) * kIdx + g;
         const bool ia = ta < M, ib = tb < M;
-        const float n4[4] = {ia ? __ldg(qa) : 0.f, ia ? __ldg(qa + 8) : 0.f, ib ? __ldg(qb) : 0.f, ib ? __ldg(qb + 8) : 0.f};
+        const float n4[4] = {ia ? __ldg(qa) : 0.f, ia ? __ldg(qa + 8) : 0.f, ib ? __ldg(qb) : 0.f,
+                             ib ? __ldg(qb + 8) : 0.f};
 #pragma unroll
         for (int e = 0; e < 4; ++e) tf32_split(n4[e], nh[e], nl[e]);
         const float4 va = ds4<kVec>(ds, ta, M, b0 + 4 * g, NB), vb = ds4<kVec>(ds, tb, M, b0 + 4 * g, NB);
@@ -722,7 +726,8 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
   const int d0 = (blockIdx.x * wd + dw) * 64, dl = d0 + 8 * g;
   uint8_t* xs = ring + warp * kXStages * kXTileBytes<kCodes>;
   uint8_t* qs = ring + kXWarps * kXStages * kXTileBytes<kCodes> + warp * kXStages * 1024;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kXWarps * kXStages * (kXTileBytes<kCodes> + 1024)) + warp * kXStages;
+  uint64_t* bars =
+      reinterpret_cast<uint64_t*>(ring + kXWarps * kXStages * (kXTileBytes<kCodes> + 1024)) + warp * kXStages;
   if (lane == 0) {
     for (int k = 0; k < kXStages; ++k) mbar_init(bars + k, 1);
     fence_mbar_init();
@@ -791,7 +796,8 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
       for (int k = 0; k < 4; ++k) {
         const int row = 2 * t + (k & 1) + 8 * (k >> 1);
         if constexpr (kCodes) {  // 64-byte swizzle: 16-byte piece ^ (row / 2) % 4
-          const uint2 c = *reinterpret_cast<const uint2*>(xs + stage * 1024 + row * 64 + (((g >> 1) ^ t) << 4) + (g & 1) * 8);
+          const uint2 c = *reinterpret_cast<const uint2*>(xs + stage * 1024 + row * 64 + (((g >> 1) ^ t) << 4) +
+                                                          (g & 1) * 8);
           const float f = mx_scale((int)byte[k]);
           const float2 a = mx_unpack2((uint16_t)c.x), b = mx_unpack2((uint16_t)(c.x >> 16));
           const float2 e = mx_unpack2((uint16_t)c.y), z = mx_unpack2((uint16_t)(c.y >> 16));
@@ -845,13 +851,13 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
       parity ^= 1;
     }
   }
-  if (tile < tiles) {  // a copy did not arrive within the wait limit: drain the others, leave NaN as the result
-    for (int k = 1; k < kXStages; ++k) {
+  if (tile < tiles) {  // a copy did not arrive within the wait limit: wait once more for all, leave NaN as the result
+    for (int k = 0; k < kXStages; ++k) {
+      if (tile + k * hop < tiles) mbar_wait(bars + stage, parity, nullptr, 0);
       if (++stage == kXStages) {
         stage = 0;
         parity ^= 1;
       }
-      if (tile + k * hop < tiles) mbar_wait(bars + stage, parity, nullptr, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -882,12 +888,11 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
         red[(tw * kIdx + 8 * j + 2 * t + (e & 1)) * width + dw * 64 + 8 * g + 2 * i + (e >> 1)] = acc[i][j][e];
   __syncthreads();
   float* part = dw_part + (int64_t)blockIdx.y * kIdx * D;
-  const int db = blockIdx.x * width;
-  for (int i = threadIdx.x; i < kIdx * width; i += blockDim.x) {
-    const int j = i / width, d = i % width;
+  const int d = threadIdx.x % width, c = blockIdx.x * width + d;
+  for (int j = threadIdx.x / width; j < kIdx; j += kXWarps * 32 / width) {
     float s = 0.f;
-    for (int k = 0; k < ntw; ++k) s += red[k * kIdx * width + i];
-    if (db + d < D) part[(int64_t)j * D + db + d] = s;
+    for (int k = 0; k < ntw; ++k) s += red[(k * kIdx + j) * width + d];
+    if (c < D) part[(int64_t)j * D + c] = s;
   }
 }
 
@@ -923,7 +928,8 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
   float w[kIdx][4], acc[kIdx][4];
 #pragma unroll
   for (int j = 0; j < kIdx; ++j) {
-    const float4 v = in && dx ? __ldg(reinterpret_cast<const float4*>(wq + (int64_t)j * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 v = in && dx ? __ldg(reinterpret_cast<const float4*>(wq + (int64_t)j * D + d))
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
     w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
@@ -946,7 +952,8 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
   for (int64_t t0 = (int64_t)blockIdx.y * tokens_per_cta; t0 < t1; t0 += kFTokens) {
     const int n = (int)min((int64_t)kFTokens, t1 - t0);
     __syncthreads();
-    for (int i = threadIdx.x; i < n * 4; i += kFThreads) sq[i] = __ldg(reinterpret_cast<const float4*>(dq + t0 * kIdx) + i);
+    for (int i = threadIdx.x; i < n * 4; i += kFThreads)
+      sq[i] = __ldg(reinterpret_cast<const float4*>(dq + t0 * kIdx) + i);
     if constexpr (kCodes) {
       if (dw_part)
         for (int i = threadIdx.x; i < n * kFScales; i += kFThreads) {
@@ -1000,12 +1007,12 @@ router_x_f32_kernel(const float* __restrict__ x, const uint8_t* __restrict__ cod
     for (int e = 0; e < 4; ++e) red[(ty * kIdx + j) * width + lane * 4 + e] = acc[j][e];
   __syncthreads();
   float* part = dw_part + (int64_t)blockIdx.y * kIdx * D;
-  for (int i = threadIdx.x; i < kIdx * width; i += kFThreads) {
-    const int j = i / width, c = i % width;
-    float s = 0.f;
-    for (int k = 0; k < nty; ++k) s += red[k * kIdx * width + i];
-    if (db + c < D) part[(int64_t)j * D + db + c] = s;
-  }
+  for (int c = threadIdx.x; c < width; c += kFThreads)
+    for (int j = 0; j < kIdx; ++j) {
+      float s = 0.f;
+      for (int k = 0; k < nty; ++k) s += red[(k * kIdx + j) * width + c];
+      if (db + c < D) part[(int64_t)j * D + db + c] = s;
+    }
 }
 
 // Pass 3: out[i] = sum over the partials, 8 interleaved sums joined in order; dWq (n1 elements), then dK (n2).
@@ -1042,7 +1049,7 @@ struct BwdPlan {
   int64_t per_cta;  // pass 2: tiles of 16 tokens (bf16) or tokens (fp32)
   size_t dq, dw, dk, copy, total;
 };
-BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
+BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB, bool from_codes) {
   BwdPlan p{};
   p.dq_ctas = (int)std::min<int64_t>((M + kDqTokens - 1) / kDqTokens, kDqMaxCtas);
   int64_t units;
@@ -1065,7 +1072,7 @@ BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB) {
   p.dw = p.dq + up((size_t)((M + 15) / 16) * 1024);
   p.dk = p.dw + up((size_t)p.parts * kIdx * D * 4);
   p.copy = p.dk + up((size_t)p.dq_ctas * kIdx * NB * 4);
-  p.total = p.copy + (dtype == FP_DTYPE_BF16 && D % 16 ? up((size_t)M * D * 2) : 0);
+  p.total = p.copy + (from_codes && dtype == FP_DTYPE_BF16 && D % 16 ? up((size_t)M * D * 2) : 0);
   return p;
 }
 
@@ -1085,7 +1092,7 @@ template <typename T>
 int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t* scales, const T* wq, const T* k16,
                const float* q16, const float* rnorm, int64_t M, int D, int NB, T* dx, void* dwq, void* dk16,
                int grad_dtype, char* ws, cudaStream_t st) {
-  const BwdPlan p = bwd_plan(sizeof(T) == 2 ? FP_DTYPE_BF16 : FP_DTYPE_F32, M, D, NB);
+  const BwdPlan p = bwd_plan(sizeof(T) == 2 ? FP_DTYPE_BF16 : FP_DTYPE_F32, M, D, NB, codes != nullptr);
   void* dq = dx || dwq ? ws + p.dq : nullptr;
   float* pw = dwq ? reinterpret_cast<float*>(ws + p.dw) : nullptr;
   float* pk = dk16 ? reinterpret_cast<float*>(ws + p.dk) : nullptr;
@@ -1100,7 +1107,8 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
       const __nv_bfloat16* rows = x;
       if (codes && D % 16) {  // rows of codes that TMA cannot address: as bf16 in the workspace
         rows = reinterpret_cast<const __nv_bfloat16*>(ws + p.copy);
-        if (const int e2 = dwq ? fp_mxfp8_dequantize(codes, scales, FP_DTYPE_BF16, M * D, ws + p.copy, st) : FP_OK) return e2;
+        if (dwq)
+          if (const int rc = fp_mxfp8_dequantize(codes, scales, FP_DTYPE_BF16, M * D, ws + p.copy, st)) return rc;
         codes = nullptr;
       }
       const auto kern = codes ? router_x_kernel<true> : router_x_kernel<false>;
@@ -1109,10 +1117,10 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
       if (dwq && !(codes ? encode_map_2d_u8(&map, codes, D, M, D, 64, 16)
                          : encode_map_2d(&map, rows, D, M, (uint64_t)D * 2, 64, 16)))
         return FP_ERR_CUDA;
-      if (!(codes ? allow_smem<router_x_kernel<true>>(smem) : allow_smem<router_x_kernel<false>>(smem))) return FP_ERR_CUDA;
+      if (!(codes ? allow_smem<router_x_kernel<true>>(smem) : allow_smem<router_x_kernel<false>>(smem)))
+        return FP_ERR_CUDA;
       e = launch_pdl(kern, grid, kXWarps * 32, smem, st, map, scales, (const uint4*)dq, wq, M, D, p.wide, dx, pw);
-    }
-    else
+    } else
       e = launch_pdl(codes ? router_x_f32_kernel<true> : router_x_f32_kernel<false>, grid, kFThreads, 0, st, x, codes,
                      scales, (const float*)dq, wq, M, D, p.wide, p.per_cta, dx, pw);
     if (e != cudaSuccess) return FP_ERR_CUDA;
@@ -1232,10 +1240,10 @@ __device__ __forceinline__ bool bal_exp(float (&z)[kE], int base, float c, int l
 // Per cluster: column sums of p over its rows, the number of counted rows, and the blocks' slot counts.
 // scores may be NULL (counts only); idx may be NULL (counts given).
 //
-// Counting: shared-memory atomics and plain byte flags take about the same time here, but flags need a third of
-// the instructions.  A row's list sets one byte per block in the warp's own shared memory; each lane adds the
-// four columns of its words to byte counters in registers (spilled to the CTA's counts every 255 rows) and
-// clears them.  A list that names a block twice is noticed by its sum and counted with atomics.
+// Counting: a row's list sets one byte per block in the warp's own shared memory; each lane adds the four columns
+// of its words to byte counters in registers (spilled to the CTA's counts before they can pass 255) and clears
+// them.  A list that names a block twice is noticed by its sum and counted with atomics.  With an atomic for
+// every entry the counts alone took 89 us at 65521 rows of up to 112, this way 49 (296 CTAs both; now 35).
 template <int kE, bool kVec>
 __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalWarps * 32, kE <= 16 ? 2 : 1)
 balance_partial_kernel(const float* __restrict__ scores, int64_t M, int NB, int base, float temperature,
@@ -1576,7 +1584,7 @@ int fp_router_scores_train(const void* x, const void* q_proj, const void* block_
                            int NB, float* scores, float* q16, float* rnorm, void* codes, void* scales, void* stream) {
   if (dtype != FP_DTYPE_F32 && dtype != FP_DTYPE_BF16) return FP_ERR_UNSUPPORTED;
   if (M < 0 || D <= 0 || NB <= 0) return FP_ERR_INVALID_ARG;
-  if (D % 8 != 0 || NB > 1024 || M > (int64_t)INT32_MAX / 8) return FP_ERR_UNSUPPORTED;
+  if (D % 8 != 0 || D > kMaxWidth || NB > 1024 || M > (int64_t)INT32_MAX / 8) return FP_ERR_UNSUPPORTED;
   if ((codes == nullptr) != (scales == nullptr)) return FP_ERR_INVALID_ARG;
   if (M == 0) return FP_OK;
   if (!x || !q_proj || !block_keys || !scores || !q16 || !rnorm) return FP_ERR_INVALID_ARG;
@@ -1594,8 +1602,8 @@ int fp_router_scores_train(const void* x, const void* q_proj, const void* block_
   return codes ? fp_mxfp8_quantize(x, dtype, M * D, codes, scales, stream) : FP_OK;
 }
 
-size_t fp_router_scores_bwd_workspace_size(int dtype, int64_t M, int D, int NB) {
-  return M > 0 && D > 0 && NB > 0 ? bwd_plan(dtype, M, D, NB).total : 256;
+size_t fp_router_scores_bwd_workspace_size(int dtype, int64_t M, int D, int NB, int from_codes) {
+  return M > 0 && D > 0 && NB > 0 ? bwd_plan(dtype, M, D, NB, from_codes != 0).total : 256;
 }
 
 int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes, const void* scales,
@@ -1605,14 +1613,14 @@ int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes,
   if (dtype != FP_DTYPE_F32 && dtype != FP_DTYPE_BF16) return FP_ERR_UNSUPPORTED;
   if (grad_dtype != FP_DTYPE_F32 && grad_dtype != FP_DTYPE_BF16) return FP_ERR_UNSUPPORTED;
   if (M <= 0 || D <= 0 || NB <= 0) return FP_ERR_INVALID_ARG;
-  if (D % 8 != 0 || NB > 1024 || M > (int64_t)INT32_MAX / 8) return FP_ERR_UNSUPPORTED;
+  if (D % 8 != 0 || D > kMaxWidth || NB > 1024 || M > (int64_t)INT32_MAX / 8) return FP_ERR_UNSUPPORTED;
   if (!dscores || !q_proj || !block_keys || !q16 || !rnorm || !workspace) return FP_ERR_INVALID_ARG;
   if (dq_proj && !x && !codes) return FP_ERR_INVALID_ARG;
   if ((codes == nullptr) != (scales == nullptr)) return FP_ERR_INVALID_ARG;
   if (!al16(x) || !al16(codes) || !al16(q_proj) || !al16(block_keys) || !al16(dx) || !al16(dscores) || !al16(q16) ||
       !al16(workspace))
     return FP_ERR_INVALID_ARG;
-  if (workspace_bytes < bwd_plan(dtype, M, D, NB).total) return FP_ERR_WORKSPACE;
+  if (workspace_bytes < bwd_plan(dtype, M, D, NB, codes != nullptr).total) return FP_ERR_WORKSPACE;
   int sms;
   if (const int rc = device_info(sms)) return rc;
   cudaStream_t st = (cudaStream_t)stream;

@@ -306,7 +306,7 @@ def router_scores_bwd(dscores: torch.Tensor, x: Optional[torch.Tensor], buf: Opt
         return (dx, torch.zeros_like(q_proj) if dw is not None else None,
                 torch.zeros_like(block_keys) if dk is not None else None)
     lib = _lib.load()
-    nbytes = lib.fp_router_scores_bwd_workspace_size(dt, M, D, NB)
+    nbytes = lib.fp_router_scores_bwd_workspace_size(dt, M, D, NB, buf is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     codes, scales = _mx_addrs(buf, M * D) if buf is not None else (None, None)
     q16 = saved.data_ptr()

@@ -465,7 +465,7 @@ FP_API int fp_swiglu_bwd_mxfp8(const void* dout, const void* g_codes, const void
 /*
  * fp_router_scores for training: the same scores, and what their gradient needs: q16 [M, 16] fp32 normalised
  * queries, rnorm [M] fp32 factors 1 / rms(x . q_proj^T) and, unless codes and scales are NULL, the MXFP8 copy
- * of x (M * D codes).
+ * of x (M * D codes).  D a multiple of 8 up to 2^24, NB <= 1024.
  */
 FP_API int fp_router_scores_train(const void* x, const void* q_proj, const void* block_keys, int dtype, int64_t M,
                                   int D, int NB, float* scores, float* q16, float* rnorm, void* codes, void* scales,
@@ -477,9 +477,10 @@ FP_API int fp_router_scores_train(const void* x, const void* q_proj, const void*
  *   dx = dq . q_proj,  dq_proj = dq^T . x,  dblock_keys = dscores^T . q16 / 4
  * dx [M, D] in `dtype`, dq_proj [16, D] and dblock_keys [NB, 16] in grad_dtype; each may be NULL (not
  * computed).  x may be NULL when codes and scales are given (its MXFP8 copy is read then, also when x is
- * given) or dq_proj is not wanted.  The sums over tokens have a fixed order.
+ * given) or dq_proj is not wanted; from_codes of the workspace size says whether codes will be.  The sums over
+ * tokens have a fixed order.
  */
-FP_API size_t fp_router_scores_bwd_workspace_size(int dtype, int64_t M, int D, int NB);
+FP_API size_t fp_router_scores_bwd_workspace_size(int dtype, int64_t M, int D, int NB, int from_codes);
 FP_API int fp_router_scores_bwd(const float* dscores, const void* x, const void* codes, const void* scales,
                                 const void* q_proj, const void* block_keys, const float* q16, const float* rnorm,
                                 int dtype, int64_t M, int D, int NB, void* dx, void* dq_proj, void* dblock_keys,

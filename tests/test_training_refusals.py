@@ -155,17 +155,20 @@ def test_c_router(lib):
     assert f(A, A, A, 1, -1, 64, 8, A, A, A, None, None, None) == INVALID
     assert f(A, A, A, 1, 4, 60, 8, A, A, A, None, None, None) == UNSUPPORTED
     assert f(A, A, A, 1, 4, 64, 1025, A, A, A, None, None, None) == UNSUPPORTED
+    assert f(A, A, A, 1, 4, 2 ** 24 + 8, 8, A, A, A, None, None, None) == UNSUPPORTED
     assert f(A, A, A, 5, 4, 64, 8, A, A, A, None, None, None) == UNSUPPORTED
     assert f(A, A, A, 1, 4, 64, 8, A, A, A, A, None, None) == INVALID
     assert f(A, A, A, 1, 4, 64, 8, A, A, A, ODD, A, None) == INVALID
-    n = w(1, 4, 64, 8)
-    assert n > 0 and w(1, 0, 0, 0) > 0
+    n = w(1, 4, 64, 8, 0)
+    assert n > 0 and w(1, 0, 0, 0, 0) > 0
+    assert w(1, 4096, 1000, 8, 1) >= w(1, 4096, 1000, 8, 0) + 4096 * 1000 * 2  # rows of codes that need a copy
 
     def go(ds=A, x=A, c=None, s=None, wq=A, k=A, q=A, r=A, dt=1, M=4, D=64, NB=8, dx=A, dw=A, dk=A, gd=0, ws=A, nb=n):
         return b(ds, x, c, s, wq, k, q, r, dt, M, D, NB, dx, dw, dk, gd, ws, nb, None)
 
     assert go(M=0) == INVALID
     assert go(D=12) == UNSUPPORTED
+    assert go(D=2 ** 24 + 8) == UNSUPPORTED
     assert go(NB=2000) == UNSUPPORTED
     assert go(dt=4) == UNSUPPORTED
     assert go(gd=4) == UNSUPPORTED
