@@ -155,11 +155,14 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.base, ctx.temperature = base, temperature
         ctx.save_for_backward(scores, valid, state)
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)  # no zeros for the counts' gradient, which would be a launch
         return loss, counts
 
     @staticmethod
     @once
     def backward(ctx, dloss, _dcounts):
+        if dloss is None:
+            return (None,) * 7
         scores, valid, state = ctx.saved_tensors
         ds = kernels.balance_loss_bwd(scores, ctx.base, ctx.temperature, valid, state, dloss)
         return ds, None, None, None, None, None, None
