@@ -588,7 +588,7 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
     const int64_t tok0 = base + 8 * warp;
     // (a tile of 16 tokens that ends past M is written whole: zeros behind the last token)
     if (for_dq && tok0 < (M + 15) / 16 * 16) {
-      float c[4] = {}, cl[4] = {};
+      float a[4] = {};
       float n0[2], n1[2], r[2];  // of tokens 2 t and 2 t + 1
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -600,34 +600,42 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
           r[e] = __ldg(rnorm + tok);
         }
       }
-#pragma unroll 8
-      for (int k = 0; k < nk; ++k) {
-        const float4 v = ds4<kVec>(ds, tok0 + g, M, 16 * k + 4 * t, NB);
+      // The tensor cores round a sum towards zero: chains of 8 steps, joined by ordinary additions (one chain over
+      // 1000 blocks left errors of 3e-6, this way 5e-7).
+      for (int k0 = 0; k0 < nk; k0 += 8) {
+        float c[4] = {}, cl[4] = {};
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const float4 kv = sk[(k * 2 + s) * 32 + lane];
-          const float kf[4] = {kv.x, kv.y, kv.z, kv.w};
-          uint32_t kh[4], kl[4];
+        for (int i = 0; i < 8; ++i) {
+          const int k = k0 + i < nk ? k0 + i : nk;  // step nk: columns past the end, zeros
+          const float4 v = ds4<kVec>(ds, tok0 + g, M, 16 * k + 4 * t, NB);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (sizeof(T) == 4) tf32_split(kf[e], kh[e], kl[e]);
-            else kh[e] = __float_as_uint(kf[e]);  // a bf16 value is a tf32 value
+          for (int s = 0; s < 2; ++s) {
+            const float4 kv = sk[(min(k, nk - 1) * 2 + s) * 32 + lane];
+            const float kf[4] = {kv.x, kv.y, kv.z, kv.w};
+            uint32_t kh[4], kl[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (sizeof(T) == 4) tf32_split(kf[e], kh[e], kl[e]);
+              else kh[e] = __float_as_uint(kf[e]);  // a bf16 value is a tf32 value
+            }
+            uint32_t h0, l0, h1, l1;
+            tf32_split(s ? v.z : v.x, h0, l0);
+            tf32_split(s ? v.w : v.y, h1, l1);
+            mma_tf32(cl, kh, l0, l1);
+            if constexpr (sizeof(T) == 4) mma_tf32(cl, kl, h0, h1);
+            mma_tf32(c, kh, h0, h1);
           }
-          uint32_t h0, l0, h1, l1;
-          tf32_split(s ? v.z : v.x, h0, l0);
-          tf32_split(s ? v.w : v.y, h1, l1);
-          mma_tf32(cl, kh, l0, l1);
-          if constexpr (sizeof(T) == 4) mma_tf32(cl, kl, h0, h1);
-          mma_tf32(c, kh, h0, h1);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += c[e] + cl[e];
       }
-      // c: token 2 t (+1: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
+      // a: token 2 t (+1: odd element), j = g (elements 0, 1) and g + 8 (2, 3)
       float d[2][2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t tok = tok0 + 2 * t + e;
         const bool in = tok < M;
-        const float a0 = (c[e] + cl[e]) * 0.25f, a1 = (c[2 + e] + cl[2 + e]) * 0.25f;
+        const float a0 = a[e] * 0.25f, a1 = a[2 + e] * 0.25f;
         float dot = a0 * n0[e] + a1 * n1[e];
         dot += __shfl_xor_sync(0xffffffffu, dot, 4);
         dot += __shfl_xor_sync(0xffffffffu, dot, 8);
