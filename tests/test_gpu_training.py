@@ -726,6 +726,29 @@ def test_captured_and_replayed():
     assert same(outs[0], step(*new)) and same(outs[1], ref[id(b)])
 
 
+def test_captured_while_an_eager_graph_lives():
+    """A pass captured on leaves of its own (the same memory) while an eager graph of the originals is alive; both
+    give what they give alone.  (On the originals themselves PyTorch's accumulation nodes, which keep the eager
+    graph's stream, end the capture with an error, whatever the operator.)"""
+    ins = step_inputs(130)
+    ref = step(*ins)
+    x, wq, k16, idx, cnt, g, u, dh = ins
+    loss, _ = fsi.balance_loss(fsi.router_scores(x, wq, k16), idx, cnt, base_blocks=2)
+    h = fsi.triton_fused_swiglu(g, u, checkpoint="mxfp8")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*[t.detach().requires_grad_(t.requires_grad) for t in ins])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert same(out, ref)
+    torch.autograd.backward([loss, h], [torch.ones_like(loss), dh])
+    assert torch.equal(g.grad, ref[7]) and torch.equal(u.grad, ref[8]) and torch.equal(x.grad, ref[4])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert same(out, ref)
+
+
 def test_two_host_threads():
     """Two threads with streams of their own give what each gives alone."""
     import threading
