@@ -12,14 +12,17 @@ namespace {
 
 // All four kernels stream: a thread takes a few vectors of 16 bytes, a CTA's width apart, and issues all of their
 // loads before the first use.  HBM bound, but for the SwiGLU forward, which the exact division and exponential
-// of fp_swiglu_fwd (whose bits it keeps) hold at 0.92 of a copy's rate: with the hardware's approximations
-// it took 278 us where it takes 318 (16384 x 14336 bf16).  Vectors to a thread, measured there (GB/s moved;
-// torch's copy 6500): copy 4 / 8: 6470 / 6810 (fp32, 16384 x 4096: 47 / 52 us); restore 2 / 4: 6680 / 6310; forward 1 / 2 / 4: 5470 / 5960 /
-// 5020; backward 1 / 2 / 4: 5970 / 5650 / 4800.  256 threads; 512 lost 5 to 15 %, 128 gained nothing sure.
+// of fp_swiglu_fwd (whose bits it keeps) hold at 0.92 of a copy's rate: with the hardware's approximations it
+// took 278 us where it takes 318 (16384 x 14336 bf16).  Vectors to a thread, measured there (GB/s moved; torch's
+// copy 6500): copy 4 / 8: 6470 / 6810 (fp32, 16384 x 4096: 47 / 52 us); restore 2 / 4: 6680 / 6310; forward
+// 1 / 2 / 4: 5470 / 5960 / 5020; backward 1 / 2 / 4: 5970 / 5650 / 4800 (fp32, 16384 x 1536: 71 / 65 us for 1 / 2).
+// 256 threads; 512 lost 5 to 15 %, 128 gained nothing sure.
 constexpr int kThreads = 256;
 template <typename T>
 constexpr int kUnrollCopy = sizeof(T) == 2 ? 8 : 4;
-constexpr int kUnrollRestore = 2, kUnrollFwd = 2, kUnrollBwd = 1;
+template <typename T>
+constexpr int kUnrollBwd = sizeof(T) == 2 ? 1 : 2;
+constexpr int kUnrollRestore = 2, kUnrollFwd = 2;
 
 template <typename T, int U>
 __device__ __forceinline__ int64_t first_element() {
@@ -101,17 +104,17 @@ swiglu_bwd_mxfp8_kernel(const T* __restrict__ dout, const uint8_t* __restrict__ 
                         const uint8_t* __restrict__ uc, const uint8_t* __restrict__ us, int64_t n,
                         T* __restrict__ dg, T* __restrict__ du, T* __restrict__ h) {
   using V = MxVec<T>;
-  const int64_t i0 = first_element<T, kUnrollBwd>();
-  uint4 dw[kUnrollBwd];
-  typename V::Codes gq[kUnrollBwd], uq[kUnrollBwd];
+  const int64_t i0 = first_element<T, kUnrollBwd<T>>();
+  uint4 dw[kUnrollBwd<T>];
+  typename V::Codes gq[kUnrollBwd<T>], uq[kUnrollBwd<T>];
 #pragma unroll
-  for (int k = 0; k < kUnrollBwd; ++k) {
+  for (int k = 0; k < kUnrollBwd<T>; ++k) {
     dw[k] = V::load(dout, i0 + k * kStep<T>, n);
     gq[k] = V::load_codes(gc, gs, i0 + k * kStep<T>, n);
     uq[k] = V::load_codes(uc, us, i0 + k * kStep<T>, n);
   }
 #pragma unroll
-  for (int k = 0; k < kUnrollBwd; ++k) {
+  for (int k = 0; k < kUnrollBwd<T>; ++k) {
     const int64_t i = i0 + k * kStep<T>;
     float d[V::kV], gv[V::kV], uv[V::kV];
     V::unpack(dw[k], d);
@@ -217,7 +220,7 @@ int fp_swiglu_bwd_mxfp8(const void* dout, const void* g_codes, const void* g_sca
   if (!al16(dout) || !al16(dg) || !al16(du) || !al16(h) || !al16(g_codes) || !al16(u_codes)) return FP_ERR_INVALID_ARG;
   return by_type(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned grid = grid_for<T>(n, kUnrollBwd);
+    const unsigned grid = grid_for<T>(n, kUnrollBwd<T>);
     if (!grid) return FP_ERR_UNSUPPORTED;
     swiglu_bwd_mxfp8_kernel<T><<<grid, kThreads, 0, (cudaStream_t)stream>>>(
         (const T*)dout, (const uint8_t*)g_codes, (const uint8_t*)g_scales, (const uint8_t*)u_codes,
