@@ -1159,6 +1159,11 @@ constexpr int kBalWarps = 16;
 constexpr int kBalCluster = 8;
 constexpr int kBalMaxCtas = 256;
 constexpr int kGradWarps = 8;
+// Temperatures: beyond these log2(e) / T or R / (T n) overflows or vanishes in 32 bits, and 0 * inf is NaN.
+constexpr bool bal_temperature(float t) { return t >= 1e-30f && t <= 1e30f; }
+// A list's longest form.  A cluster's slot count of one block has 32 bits: rows of one name only, 2^20 of them to
+// a row, pass it with 2^31 entries to a cluster, 2^36 in all (256 GB).
+constexpr int kBalMaxCapacity = 1 << 20;
 
 template <int kE>
 constexpr int kRowsOf = kE <= 4 ? 4 : kE == 8 ? 2 : 1;
@@ -1282,7 +1287,7 @@ balance_partial_kernel(const float* __restrict__ scores, int64_t M, int NB, int 
   for (int i = 0; i < kE; ++i) acc[i] = 0.f;
   uint32_t slots[kW] = {};
   int pending = 0, counted = 0;
-  const float c = fminf(__fdiv_rn(1.4426950408889634f, temperature), 3.4028234663852886e38f);
+  const float c = __fdiv_rn(1.4426950408889634f, temperature);
   const int64_t step = (int64_t)gridDim.x * kBalWarps;
   const bool lists = idx != nullptr;
   for (int64_t t0 = (int64_t)blockIdx.x * kBalWarps + warp;; t0 += step * kR) {
@@ -1471,7 +1476,7 @@ balance_grad_kernel(const float* __restrict__ scores, int64_t M, int NB, int bas
   constexpr int kHead = kVec ? 4 : 4 < kE ? 4 : kE;
   const int lane = threadIdx.x & 31;
   const float scale = state[NB] * *dloss;
-  const float c = fminf(__fdiv_rn(1.4426950408889634f, temperature), 3.4028234663852886e38f);
+  const float c = __fdiv_rn(1.4426950408889634f, temperature);
   float f[kE];
 #pragma unroll
   for (int i = 0; i < kE; ++i) f[i] = bal_col<kVec>(lane, i) < NB ? state[bal_col<kVec>(lane, i)] : 0.f;
@@ -1654,7 +1659,8 @@ int fp_balance_loss_fwd(const float* scores, int64_t M, int NB, int base_blocks,
   if (NB > 1024 || M > (int64_t)INT32_MAX / 8) return FP_ERR_UNSUPPORTED;
   if ((remote_indices == nullptr) != (remote_counts == nullptr)) return FP_ERR_INVALID_ARG;
   if ((loss == nullptr) != (state == nullptr)) return FP_ERR_INVALID_ARG;
-  if (loss && ((M > 0 && !scores) || base_blocks >= NB || !(temperature > 0.f))) return FP_ERR_INVALID_ARG;
+  if (capacity > kBalMaxCapacity) return FP_ERR_UNSUPPORTED;
+  if (loss && ((M > 0 && !scores) || base_blocks >= NB || !bal_temperature(temperature))) return FP_ERR_INVALID_ARG;
   if (!loss && !counts) return FP_ERR_INVALID_ARG;
   if (M > 0 && !remote_indices && !counts_in) return FP_ERR_INVALID_ARG;
   if (!workspace || !al16(workspace)) return FP_ERR_INVALID_ARG;
@@ -1682,7 +1688,8 @@ int fp_balance_loss_fwd(const float* scores, int64_t M, int NB, int base_blocks,
 
 int fp_balance_loss_bwd(const float* scores, int64_t M, int NB, int base_blocks, float temperature,
                         const uint8_t* valid, const float* state, const float* dloss, float* dscores, void* stream) {
-  if (M < 0 || NB <= 0 || base_blocks < 0 || base_blocks >= NB || !(temperature > 0.f)) return FP_ERR_INVALID_ARG;
+  if (M < 0 || NB <= 0 || base_blocks < 0 || base_blocks >= NB || !bal_temperature(temperature))
+    return FP_ERR_INVALID_ARG;
   if (NB > 1024 || M > (int64_t)INT32_MAX / 8) return FP_ERR_UNSUPPORTED;
   if (M == 0) return FP_OK;
   if (!scores || !state || !dloss || !dscores) return FP_ERR_INVALID_ARG;

@@ -25,6 +25,7 @@ from . import kernels
 from ._lib import dtype_code
 
 CHECKPOINTS = (None, "mxfp8")
+MAX_CAPACITY = 1 << 20  # slots of a row's route list
 
 
 def check_checkpoint(checkpoint: Optional[str]) -> Optional[str]:
@@ -122,6 +123,8 @@ def _check_routes(remote_indices: Tensor, remote_counts: Tensor) -> None:
     if remote_indices.dim() < 1 or remote_indices.shape[:-1] != remote_counts.shape:
         raise ValueError(f"shapes: remote_indices [..., capacity], remote_counts [...]; got "
                          f"{tuple(remote_indices.shape)} and {tuple(remote_counts.shape)}")
+    if remote_indices.shape[-1] > MAX_CAPACITY:  # partial slot counts have 32 bits
+        raise ValueError(f"a route list holds at most {MAX_CAPACITY} slots, got {remote_indices.shape[-1]}")
 
 
 def _check_valid(valid: Optional[Tensor], lead: torch.Size) -> None:
@@ -179,14 +182,16 @@ def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts
     the number of rows, ``loss = R sum_b f_b (1/n) sum_t p_tb``: 1 for an even load, R when one block takes
     everything.  The gradient reaches the scores through p only.
 
-    Rows whose ``valid`` is False or whose remote scores are all -inf are not counted and receive zeros.
+    Rows whose ``valid`` is False or whose remote scores are all -inf are not counted in n and receive zeros;
+    the slots are those of :func:`block_counts`, which leaves out the rows whose ``valid`` is False only.
     ``counts`` (int64 [NB], :func:`block_counts` summed over ranks) replaces the lists' own counts; the
     lists may be None then.  Returns (loss fp32 0-d, counts int64 [NB])."""
     NB = _check_blocks(scores.shape[-1] if scores.dim() else 0)
     if not 0 <= int(base_blocks) < NB:
         raise ValueError(f"base_blocks must leave a remote block: 0 <= base_blocks < {NB}, got {base_blocks}")
-    if not 0.0 < float(temperature) < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    # beyond these the kernels' fp32 1 / T and R / (T n) would overflow or vanish, and 0 * inf be NaN
+    if not 1e-30 <= float(temperature) <= 1e30:
+        raise ValueError(f"temperature must be between 1e-30 and 1e30, got {temperature}")
     if not scores.is_floating_point():
         raise TypeError(f"scores must be floating point, got {scores.dtype}")
     lead = scores.shape[:-1]

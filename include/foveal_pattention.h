@@ -495,7 +495,8 @@ FP_API int fp_router_scores_bwd(const float* dscores, const void* x, const void*
  *   loss = R * sum_b f_b * (1/n) sum_t p_tb                               (0 when no row is counted)
  * counts_in [NB] (optional) replaces the lists' own counts, for example summed over ranks.  loss and state
  * [NB + 1] NULL: counts only (scores are not read).  fp_balance_loss_bwd: dscores from the state and the
- * device scalar dloss; base columns and rows that are not counted receive zeros.  NB <= 1024.
+ * device scalar dloss; base columns and rows that are not counted receive zeros.  NB <= 1024, capacity
+ * <= 2^20, 1e-30 <= T <= 1e30.
  */
 FP_API size_t fp_balance_workspace_size(int64_t M, int NB);
 FP_API int fp_balance_loss_fwd(const float* scores, int64_t M, int NB, int base_blocks, float temperature,

@@ -89,6 +89,21 @@ def test_balance_loss_values(kw):
         fsi.balance_loss(torch.zeros(4, 8), idx, cnt, **kw)
 
 
+@pytest.mark.parametrize("temperature", [1e300, 3.5e38, 1e31, 1e-31, 1e-60])
+def test_balance_loss_temperature_range(temperature):
+    idx, cnt = _routes()
+    with pytest.raises(ValueError, match="temperature"):
+        fsi.balance_loss(torch.zeros(4, 8), idx, cnt, base_blocks=0, temperature=temperature)
+
+
+def test_route_list_too_long():
+    idx, cnt = torch.zeros(1, 1, dtype=torch.int32).expand(4, 2 ** 20 + 1), _routes()[1]
+    with pytest.raises(ValueError, match="slots"):
+        fsi.block_counts(idx, cnt, 8)
+    with pytest.raises(ValueError, match="slots"):
+        fsi.balance_loss(torch.zeros(4, 8), idx, cnt, base_blocks=0)
+
+
 def test_balance_loss_shapes_and_dtypes():
     idx, cnt = _routes()
     s = torch.zeros(4, 8)
@@ -211,3 +226,15 @@ def test_c_balance(lib):
         args = [A, 4, 8, 1, 1.0, None, A, A, A, None]
         args[k] = None
         assert b(*args) == INVALID, k
+
+
+def test_c_balance_limits(lib):
+    f, b, n = lib.fp_balance_loss_fwd, lib.fp_balance_loss_bwd, lib.fp_balance_workspace_size(4, 8)
+
+    def go(T=1.0, cap=2):
+        return f(A, 4, 8, 1, T, None, A, A, cap, None, A, A, A, A, n, None)
+
+    for T in (float("inf"), 1e31, 1e-31):
+        assert go(T=T) == INVALID
+        assert b(A, 4, 8, 1, T, None, A, A, A, None) == INVALID
+    assert go(cap=2 ** 20 + 1) == UNSUPPORTED
