@@ -1210,7 +1210,9 @@ __device__ __forceinline__ float warp_max(float v) {
 // the lane's part of their sum.  Returns whether the row is counted: a row whose remote scores are all -inf
 // has no distribution and is not; a NaN makes the whole row NaN.  c = log2(e) / T.  The passes are issue bound
 // at 448 blocks (24 instructions a score before, about 7 now), hence one fused multiply-add and the hardware
-// exponential per score: 2^-22 of p, next to the rounding of z c (|z| c 2^-24).
+// exponential per score: 2^-22 of p, next to the rounding of z c (|z| c 2^-24).  The rounding of `d` is the same for
+// a whole row and leaves p as it is, but it shifts the exponents by up to |d| 2^-24: from |d| = 2^20 on (a row of
+// -1e30 as a mask, a temperature near 0) the difference to the largest score is taken first.
 template <int kE, bool kVec>
 __device__ __forceinline__ bool bal_exp(float (&z)[kE], int base, float c, int lane, float& sum) {
   constexpr int kHead = kVec ? 4 : 4 < kE ? 4 : kE;  // elements in a lane's first 128 columns
@@ -1228,10 +1230,10 @@ __device__ __forceinline__ bool bal_exp(float (&z)[kE], int base, float c, int l
   top = warp_max(top);
   const float d = -top * c;
   sum = 0.f;
-  if (fabsf(d) <= 1e38f) {
+  if (fabsf(d) <= 0x1p20f) {
 #pragma unroll
     for (int i = 0; i < kE; ++i) z[i] = exp2_fast(fmaf(z[i], c, d));
-  } else {  // nothing above -inf, an infinity, or scores of the type's lowest value (a mask) only
+  } else {  // large scores, an infinity, a NaN, or nothing above -inf
     if (top == -INFINITY) {
       bool nan = false;
 #pragma unroll
@@ -1240,10 +1242,7 @@ __device__ __forceinline__ bool bal_exp(float (&z)[kE], int base, float c, int l
       top = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      const float e = z[i] - top;  // equal scores: exactly 0
-      z[i] = e == 0.f ? 1.f : exp2_fast(e * c);
-    }
+    for (int i = 0; i < kE; ++i) z[i] = exp2_fast((z[i] - top) * c);
   }
 #pragma unroll
   for (int i = 0; i < kE; ++i) sum += z[i];

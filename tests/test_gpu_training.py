@@ -925,3 +925,51 @@ def test_training_step_of_all(dtype):
     (out_loss() + 0.01 * m.balance_loss(x)[0]).backward()
     assert all(bool(torch.isfinite(p.grad).all()) for p in m.parameters())
     assert int(counts.sum()) >= 4 * 33
+
+
+def check_balance_by_differences(s, idx, cnt, base, T):
+    """Against the reference with the tolerance of scores whose largest is 0: p depends on differences only."""
+    loss, counts, ds = run_balance(s, idx, cnt, base, temperature=T)
+    top = s[:, base:].amax(dim=1, keepdim=True)
+    shifted = s.double() - torch.where(top.isfinite(), top, 0.0).double()
+    ref, rc, rds, _, _ = balance_ref(s, idx, cnt, base, T)
+    z = shifted[:, base:] / T
+    # exp2's argument: |z| steps of c, of the difference and of the product; beyond 150 p is below 2^-200
+    zmax = torch.where(z.abs() < 150, z.abs(), 0.0).amax(dim=1, keepdim=True)
+    rows = ~(s[:, base:] == -math.inf).all(dim=1)
+    p = torch.where(rows[:, None], torch.softmax(z, dim=1), 0.0)
+    R, n, M = s.shape[1] - base, int(rows.sum()), s.shape[0]
+    f = counts[base:].double() / int(counts.sum())
+    g, c = (f - 1.0 / R).abs(), 4 * zmax + s.shape[1] + 40
+    tol = torch.zeros_like(rds)
+    tol[:, base:] = p * (g + (p * g).sum(dim=1, keepdim=True)) * R / (T * n) * c * U
+    assert torch.equal(counts, rc)
+    assert abs(float(loss) - float(ref)) <= float((R * p * f * (c + M / 8 + 16)).sum() / n) * U + U * float(ref)
+    check(ds, rds, tol + U * rds.abs() + 1e-37)
+
+
+@pytest.mark.parametrize("at", [0.0, 2.0 ** 18, -2.0 ** 20, 2.0 ** 22, -2.0 ** 40, 1e12, -1e30, 2.0 ** 105, -2.0 ** 120])
+@pytest.mark.parametrize("unit", [False, True])
+def test_balance_loss_large_scores(at, unit):
+    """Rows whose scores are all large, a few steps of fp32 apart: temperature 1, and the temperature of one step."""
+    M, NB, base = 90, 100, 3
+    s, idx, cnt = balance_case(M, NB, base, 6)
+    k = torch.randint(0, 5, (M, NB), generator=gen(61), device=DEV).double()
+    step = max(torch.finfo(torch.float32).eps * 2 * abs(at), 2.0 ** -23)
+    s = (at + k * step).float()
+    s[:, :base] = 7.0
+    s[5, 10:60] = -math.inf
+    s[6, base:] = -math.inf
+    s[7, 20] += 8 * step
+    T = 1.0 if unit else step
+    check_balance_by_differences(s, idx, cnt, base, T)
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e-6, 1e8, 1e30])
+def test_balance_loss_extreme_temperatures(T):
+    """Smallest: one block takes each row.  Largest: all alike, and finfo.min still a mask."""
+    s, idx, cnt = balance_case(70, 100, 2, 6)
+    s[3, 5:90] = -math.inf
+    s[4] = -math.inf
+    s[5, 40:] = torch.finfo(torch.float32).min
+    check_balance_by_differences(s, idx, cnt, 2, T)
