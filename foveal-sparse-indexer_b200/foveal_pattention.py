@@ -330,7 +330,8 @@ class FovealPattentionMLP(nn.Module):
 
         The routes are the ones ``routing="token"`` takes (``top_p``, ``min_remote_blocks``,
         ``max_remote_blocks``); the loss reaches x, q_proj_16d and block_keys_16d through the router scores.
-        ``valid`` (bool [...]) leaves out padding.  Add a small multiple to the training loss to keep the
+        ``valid`` (bool [...]) leaves out padding, whose rows of x have to be finite all the same where a
+        gradient is taken (0 times NaN is NaN in the router's own backward pass).  Add a small multiple to the training loss to keep the
         blocks' loads even; see :func:`training.balance_loss`."""
         xx = x.to(self.k_gate.dtype)
         scores = router_scores(xx, self.q_proj_16d.weight, self.block_keys_16d, checkpoint=self.checkpoint)
