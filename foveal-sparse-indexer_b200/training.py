@@ -180,7 +180,7 @@ def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts
     remote_counts [...] the routes chosen from them (``select_blocks``).  With p_t the softmax of
     scores_t / temperature over the R = NB - base_blocks remote blocks, f_b block b's share of the slots and n
     the number of rows, ``loss = R sum_b f_b (1/n) sum_t p_tb``: 1 for an even load, R when one block takes
-    everything.  The gradient reaches the scores through p only.
+    everything.  Temperatures from 1e-30 to 1e30, at most 2^20 slots to a list.  The gradient reaches the scores through p only.
 
     Rows whose ``valid`` is False or whose remote scores are all -inf are not counted in n and receive zeros;
     the slots are those of :func:`block_counts`, which leaves out the rows whose ``valid`` is False only.
