@@ -490,8 +490,9 @@ int launch_router_fwd(const void* x, const void* wq, const void* k16, int64_t M,
 // an eighth, mma.sync fits: the 16 router dimensions are its m (pass 1) and its k or two n-tiles (pass 2).
 //
 // Precision.  Pass 1 multiplies fp32 values as tf32 pieces, v = hi + lo (the rest is below 2^-22 of v):
-// hi hi + hi lo + lo hi, fp32 accumulators.  Pass 2 with bf16 x holds dq as two bf16 pieces (rest below
-// 2^-17 of dq, against 2^-8 for the bf16 gradients), x and Wq are exact.  fp32 x stays on the FMA units.
+// hi hi + hi lo + lo hi, fp32 accumulators.  Pass 2 with bf16 x holds dq as three bf16 pieces, which together are
+// all of its 24 bits (two left errors of 2.5e-6 in dWq and moved one in 450 roundings of dx); x and Wq are
+// exact.  fp32 x stays on the FMA units.
 //
 // Fragment coordinates below: lane = 4 g + t, g = 0..7, t = 0..3.
 
@@ -540,13 +541,15 @@ __device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, i
 constexpr int kDqWarps = 8;
 constexpr int kDqTokens = 8 * kDqWarps;  // tokens of a CTA's tile
 constexpr int kDqMaxCtas = 296;
+constexpr int kDqPieces = 3;                  // bf16 pieces of a packed dq
+constexpr int kDqTileBytes = kDqPieces * 512;  // 16 tokens of them
 
 // Pass 1.  CTAs of two kinds, running side by side (one after the other in each CTA they took 31 us at 16384 x 448).
 // dq (blockIdx.y = 0 where dq is wanted): 8 tokens to a warp, a^T[j, tok] = K^T[j, b] dS^T[b, tok], then dq.
 // dK (the other rows of the grid, 256 blocks each): 32 blocks to a warp over the CTA's 64 tokens, dK^T[j, b] =
 // n^T[j, tok] dS[tok, b], kept in registers over all of the CTA's tiles.  The order of b within a product and
 // the columns of a tile are permuted so that a lane's elements are 16 contiguous bytes.
-// dq: kPacked, per tile of 16 tokens the two bf16 pieces as pass 2's fragments ([tile][hi, lo][lane] uint4);
+// dq: kPacked, per tile of 16 tokens the three bf16 pieces as pass 2's fragments ([tile][piece][lane] uint4);
 // otherwise fp32 [M, 16].
 template <typename T, bool kPacked, bool kVec>
 __global__ void __launch_bounds__(kDqWarps * 32)
@@ -652,15 +655,18 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
         }
       }
       if constexpr (kPacked) {
-        uint32_t hi[2], lo[2];
+        uint2* o = reinterpret_cast<uint2*>(dq_out) + (tok0 / 16) * (64 * kDqPieces) + 2 * lane + (tok0 / 8 & 1);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          hi[j] = pack_bf16(d[j][0], d[j][1]);
-          lo[j] = pack_bf16(d[j][0] - __uint_as_float(hi[j] << 16), d[j][1] - __uint_as_float(hi[j] & 0xFFFF0000u));
+        for (int k = 0; k < kDqPieces; ++k) {
+          uint32_t w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            w[j] = pack_bf16(d[j][0], d[j][1]);
+            d[j][0] -= __uint_as_float(w[j] << 16);
+            d[j][1] -= __uint_as_float(w[j] & 0xFFFF0000u);
+          }
+          o[64 * k] = make_uint2(w[0], w[1]);
         }
-        uint2* o = reinterpret_cast<uint2*>(dq_out) + (tok0 / 16) * 128 + 2 * lane + (tok0 / 8 & 1);
-        o[0] = make_uint2(hi[0], hi[1]);
-        o[64] = make_uint2(lo[0], lo[1]);
       }
     }
     if (!for_dq && b0 < NB) {
@@ -714,11 +720,12 @@ constexpr int kXWarps = 8;
 // x (or its codes) comes by TMA, 64 columns x 16 tokens a tile, and dq with it, into a ring of kXStages tiles that a
 // warp keeps for itself: one lane copies, every lane waits on the stage's mbarrier, no other barrier.  Rows
 // and columns past the end arrive as zeros.
-constexpr int kXStages = 4;
+template <bool kCodes>
+constexpr int kXStages = kCodes ? 4 : 3;  // two CTAs to an SM
 template <bool kCodes>
 constexpr int kXTileBytes = kCodes ? 1024 : 2048;
 template <bool kCodes>
-constexpr int kXSmem = kXWarps * kXStages * (kXTileBytes<kCodes> + 1024 + 8) + 1024;
+constexpr int kXSmem = kXWarps * kXStages<kCodes> * (kXTileBytes<kCodes> + kDqTileBytes + 8) + 1024;
 
 template <bool kCodes>
 __global__ void __launch_bounds__(kXWarps * 32, 2)
@@ -726,18 +733,19 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
                 const uint4* __restrict__ dq, const __nv_bfloat16* __restrict__ wq, int64_t M, int D, int wd,
                 __nv_bfloat16* __restrict__ dx, float* __restrict__ dw_part) {
   extern __shared__ uint8_t dyn[];
+  constexpr int kStages = kXStages<kCodes>;
   // [warp][stage] tiles of x, [warp][stage] tiles of dq, [warp][stage] barriers; at the end red[token group][j][wd * 64]
   uint8_t* ring = dyn + (1024 - (smem_u32(dyn) & 1023)) % 1024;  // the swizzle counts from 1024-byte boundaries
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int dw = warp % wd, tw = warp / wd, ntw = kXWarps / wd;
   const int d0 = (blockIdx.x * wd + dw) * 64, dl = d0 + 8 * g;
-  uint8_t* xs = ring + warp * kXStages * kXTileBytes<kCodes>;
-  uint8_t* qs = ring + kXWarps * kXStages * kXTileBytes<kCodes> + warp * kXStages * 1024;
+  uint8_t* xs = ring + warp * kStages * kXTileBytes<kCodes>;
+  uint8_t* qs = ring + kXWarps * kStages * kXTileBytes<kCodes> + warp * kStages * kDqTileBytes;
   uint64_t* bars =
-      reinterpret_cast<uint64_t*>(ring + kXWarps * kXStages * (kXTileBytes<kCodes> + 1024)) + warp * kXStages;
+      reinterpret_cast<uint64_t*>(ring + kXWarps * kStages * (kXTileBytes<kCodes> + kDqTileBytes)) + warp * kStages;
   if (lane == 0) {
-    for (int k = 0; k < kXStages; ++k) mbar_init(bars + k, 1);
+    for (int k = 0; k < kStages; ++k) mbar_init(bars + k, 1);
     fence_mbar_init();
   }
   uint32_t wb[8][2];
@@ -765,9 +773,9 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
   const int tile0 = blockIdx.y * ntw + tw, hop = gridDim.y * ntw;
   const auto fetch = [&](int tile, int stage) {  // lane 0
     if (tile >= tiles) return;
-    mbar_arrive_expect_tx(bars + stage, dw_part ? kXTileBytes<kCodes> + 1024 : 1024);
+    mbar_arrive_expect_tx(bars + stage, dw_part ? kXTileBytes<kCodes> + kDqTileBytes : kDqTileBytes);
     if (dw_part) tma_load_2d(xs + stage * kXTileBytes<kCodes>, &map, bars + stage, d0, tile * 16);
-    bulk_load(qs + stage * 1024, dq + (int64_t)tile * 64, 1024, bars + stage);
+    bulk_load(qs + stage * kDqTileBytes, dq + (int64_t)tile * (kDqTileBytes / 16), kDqTileBytes, bars + stage);
   };
   uint32_t byte[4] = {127u, 127u, 127u, 127u};
   int64_t at = ((int64_t)tile0 * 16 + 2 * t) * D + dl;  // element that the next scales belong to
@@ -790,14 +798,13 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
   fetch_scales(tile0);
   griddep_wait();
   if (lane == 0)
-    for (int k = 0; k < kXStages; ++k) fetch(tile0 + k * hop, k);
+    for (int k = 0; k < kStages; ++k) fetch(tile0 + k * hop, k);
   __syncwarp();  // the barriers' initialisation
   int stage = 0, tile = tile0;
   uint32_t parity = 0;
   for (; tile < tiles; tile += hop) {
     if (!__all_sync(0xffffffffu, mbar_wait(bars + stage, parity, nullptr, 0))) break;
-    const uint4* q = reinterpret_cast<const uint4*>(qs + stage * 1024);
-    const uint4 h4 = q[lane], l4 = q[32 + lane];
+    const uint4* q = reinterpret_cast<const uint4*>(qs + stage * kDqTileBytes) + lane;  // the pieces, largest first
     uint4 r[4];
     if (dw_part) {
 #pragma unroll
@@ -818,8 +825,15 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
     }
     fetch_scales(tile + hop);
     if (dx) {
-      const uint32_t ah[4] = {transpose8x8(h4.x), transpose8x8(h4.z), transpose8x8(h4.y), transpose8x8(h4.w)};
-      const uint32_t al[4] = {transpose8x8(l4.x), transpose8x8(l4.z), transpose8x8(l4.y), transpose8x8(l4.w)};
+      uint32_t a[kDqPieces][4];
+#pragma unroll
+      for (int k = 0; k < kDqPieces; ++k) {
+        const uint4 v = q[32 * k];
+        a[k][0] = transpose8x8(v.x);
+        a[k][1] = transpose8x8(v.z);
+        a[k][2] = transpose8x8(v.y);
+        a[k][3] = transpose8x8(v.w);
+      }
       const bool in_a = (int64_t)tile * 16 + g < M, in_b = (int64_t)tile * 16 + 8 + g < M;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -827,8 +841,9 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float c[4];
-          mma_bf16_zero(c, al[0], al[1], al[2], al[3], wb[4 * h + i][0], wb[4 * h + i][1]);
-          mma_bf16(c, ah[0], ah[1], ah[2], ah[3], wb[4 * h + i][0], wb[4 * h + i][1]);
+          mma_bf16_zero(c, a[2][0], a[2][1], a[2][2], a[2][3], wb[4 * h + i][0], wb[4 * h + i][1]);
+          mma_bf16(c, a[1][0], a[1][1], a[1][2], a[1][3], wb[4 * h + i][0], wb[4 * h + i][1]);
+          mma_bf16(c, a[0][0], a[0][1], a[0][2], a[0][3], wb[4 * h + i][0], wb[4 * h + i][1]);
           oa[i] = pack_bf16(c[0], c[1]);
           ob[i] = pack_bf16(c[2], c[3]);
         }
@@ -840,29 +855,33 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
       po += (int64_t)16 * hop * D;
     }
     if (dw_part) {
+      uint4 dq4[kDqPieces];  // (read again: held from above, they spill)
+#pragma unroll
+      for (int k = 0; k < kDqPieces; ++k) dq4[k] = q[32 * k];
       const uint32_t w0[4] = {r[0].x, r[0].y, r[0].z, r[0].w}, w1[4] = {r[1].x, r[1].y, r[1].z, r[1].w};
       const uint32_t w2[4] = {r[2].x, r[2].y, r[2].z, r[2].w}, w3[4] = {r[3].x, r[3].y, r[3].z, r[3].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a0 = __byte_perm(w0[i], w1[i], 0x5410), a1 = __byte_perm(w0[i], w1[i], 0x7632);
         const uint32_t a2 = __byte_perm(w2[i], w3[i], 0x5410), a3 = __byte_perm(w2[i], w3[i], 0x7632);
-        mma_bf16(acc[i][0], a0, a1, a2, a3, l4.x, l4.z);
-        mma_bf16(acc[i][1], a0, a1, a2, a3, l4.y, l4.w);
-        mma_bf16(acc[i][0], a0, a1, a2, a3, h4.x, h4.z);
-        mma_bf16(acc[i][1], a0, a1, a2, a3, h4.y, h4.w);
+#pragma unroll
+        for (int k = kDqPieces - 1; k >= 0; --k) {
+          mma_bf16(acc[i][0], a0, a1, a2, a3, dq4[k].x, dq4[k].z);
+          mma_bf16(acc[i][1], a0, a1, a2, a3, dq4[k].y, dq4[k].w);
+        }
       }
     }
-    __syncwarp();  // the tile is in every lane's registers: its place takes the tile kXStages on
-    if (lane == 0) fetch(tile + kXStages * hop, stage);
-    if (++stage == kXStages) {
+    __syncwarp();  // the tile is in every lane's registers: its place takes the tile kStages on
+    if (lane == 0) fetch(tile + kStages * hop, stage);
+    if (++stage == kStages) {
       stage = 0;
       parity ^= 1;
     }
   }
   if (tile < tiles) {  // a copy did not arrive within the wait limit: wait once more for all, leave NaN as the result
-    for (int k = 0; k < kXStages; ++k) {
+    for (int k = 0; k < kStages; ++k) {
       if (tile + k * hop < tiles) mbar_wait(bars + stage, parity, nullptr, 0);
-      if (++stage == kXStages) {
+      if (++stage == kStages) {
         stage = 0;
         parity ^= 1;
       }
@@ -1077,7 +1096,7 @@ BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB, bool from_codes) {
   p.parts = (int)((units + p.per_cta - 1) / p.per_cta);
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p.dq = 0;
-  p.dw = p.dq + up((size_t)((M + 15) / 16) * 1024);
+  p.dw = p.dq + up((size_t)((M + 15) / 16) * (dtype == FP_DTYPE_BF16 ? kDqTileBytes : 16 * kIdx * 4));
   p.dk = p.dw + up((size_t)p.parts * kIdx * D * 4);
   p.copy = p.dk + up((size_t)p.dq_ctas * kIdx * NB * 4);
   p.total = p.copy + (from_codes && dtype == FP_DTYPE_BF16 && D % 16 ? up((size_t)M * D * 2) : 0);

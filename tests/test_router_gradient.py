@@ -1,0 +1,119 @@
+"""Precision of the router scores' gradient, by norms against a 64-bit restatement.
+
+Elementwise bounds from sums of magnitudes grow faster than the gradients themselves; what the kernels' roundings
+do to a gradient as a whole is far smaller, and its norm shows a wrong or imprecise term that such bounds let
+pass.  u = 2^-24 is half a step of fp32.  A gradient's relative error in norm is taken to be at most
+``budget(D)`` = (24 + D / 256) u, the sum of
+
+* 4 u: dS as two tf32 pieces (the rest is below 2^-22 of each term);
+* 8 u: a = dS K / 4 in chains of 8 steps of the tensor cores, which round towards zero, u on average a step;
+* 8 u: the normalisation, its dot product and the projection (a rounding each of a few fp32 operations);
+* 4 u: the last product (three steps of the tensor cores, or one chain of 16 fused multiply-adds);
+* D / 256 u: the forward's projections, D / 64 truncated steps in a quarter of the width (on partial sums, which
+  grow like a square root, and of which the part common to all of a query drops out in the normalisation).
+
+dx in bf16 is compared with the reference rounded to bf16.  An error d of an element moves its rounding over a
+border with probability |d| / s, s <= 2^-7 |v| the step there, and changes it by s; the squares add up to
+sum |d| s <= 2^-7 |d| |v| in norms (Cauchy-Schwarz), so the norm of the change is sqrt(2^-7 e) |v|; three steps at
+the largest element are left for the chance in it.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import fsi
+
+kernels = fsi.kernels
+U = 2.0 ** -24
+EPS = 1.1920928955078125e-07
+SIZES = [(1, 8, 1), (1, 64, 16), (3, 72, 5), (16, 256, 16), (17, 264, 33), (64, 256, 224), (130, 1000, 65),
+         (33, 512, 1024), (257, 1024, 130), (1000, 128, 12), (700, 512, 448)]
+
+
+def budget(D):
+    return (24 + D / 256) * U
+
+
+def inputs(M, D, NB, dtype, device, seed=200):
+    """x in ``dtype``, weights of fp32 that hold values of ``dtype`` (their gradients leave in fp32), dS."""
+    g = torch.Generator(device=device).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=device)
+    x, wq, k16, ds = r(M, D), r(16, D) * D ** -0.5, r(NB, 16) * 0.25, r(M, NB)
+    return x.to(dtype), wq.to(dtype).float(), k16.to(dtype).float(), ds
+
+
+def gradient(x, xq, wq, k16, ds):
+    """(dx, dwq, dk) in 64 bits; ``xq``: the tokens that q_proj's gradient reads."""
+    x, xq, wq, k16, ds = (t.detach().double() for t in (x, xq, wq, k16, ds))
+    q = x @ wq.t()
+    r = ((q * q).mean(dim=1, keepdim=True) + EPS).rsqrt()
+    n = q * r
+    a = ds @ k16 / 4
+    dq = r * (a - n * (a * n).mean(dim=1, keepdim=True))
+    return dq @ wq, dq.t() @ xq, ds.t() @ n / 4
+
+
+def check_norms(got, ref, dtype, e):
+    """dx, dwq and dk as wholes, and dwq by router dimension, dx by token and dk by block: none may have less
+    than the average of the allowance."""
+    for name, g, r in zip(("dx", "dwq", "dk"), got, ref):
+        assert bool(torch.isfinite(g).all()), name
+        one = r.double()
+        tol = e
+        slack = 0.0
+        if name == "dx" and dtype == torch.bfloat16:
+            one = one.to(dtype).double()
+            tol = (2.0 ** -7 * e) ** 0.5 + e
+            slack = 3 * 2.0 ** -7
+        d = g.double() - one
+        assert float(d.norm()) <= tol * float(r.norm()) + slack * float(r.abs().max()), \
+            (name, float(d.norm() / r.norm()), tol)
+        rows = r.norm(dim=1).clamp_min(float(r.norm()) / r.shape[0] ** 0.5)
+        over = d.norm(dim=1) - (4 * tol * rows + slack * r.abs().amax(dim=1))
+        assert float(over.max()) <= 0, (name, int(over.argmax()), float(over.max()))
+
+
+def run(x, wq, k16, ds, checkpoint):
+    leaves = [t.clone().requires_grad_() for t in (x, wq, k16)]
+    return torch.autograd.grad(fsi.router_scores(*leaves, checkpoint=checkpoint), leaves, ds)
+
+
+def kept(x, checkpoint):
+    return fsi.checkpoint_mxfp8(x).restore() if checkpoint else x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,D,NB", SIZES)
+def test_gradient_norms(M, D, NB, dtype, checkpoint):
+    x, wq, k16, ds = inputs(M, D, NB, dtype, "cuda")
+    got = run(x, wq, k16, ds, checkpoint)
+    assert [g.dtype for g in got] == [dtype, torch.float32, torch.float32]
+    check_norms(got, gradient(x, kept(x, checkpoint), wq, k16, ds), dtype, budget(D))
+
+
+@pytest.mark.gpu
+def test_input_gradient_has_no_part_along_the_query():
+    """A token that is the d-th unit vector has the d-th column of q_proj as its query q, and dx_d = dq q, which the
+    normalisation makes 0 but for eps.  What is left are the roundings: of the factor r (twice, on the quarter
+    of a that a direction among 16 has), of the dot product and of each dq, together some u of |dq| |q|; 4 u
+    are allowed.  dq in fewer than 24 bits shows: two bf16 pieces leave 2^-18.7 / 4 = 10 u."""
+    D, NB = 64, 40
+    g = torch.Generator(device="cuda").manual_seed(210)
+    wq = torch.randint(-60, 61, (16, D), generator=g, device="cuda").to(torch.bfloat16)
+    k16 = torch.randn(NB, 16, generator=g, device="cuda").to(torch.bfloat16)
+    ds = torch.randn(8 * D, NB, generator=g, device="cuda")
+    x = torch.eye(D, device="cuda").repeat(8, 1).to(torch.bfloat16).requires_grad_()
+    dx, = torch.autograd.grad(fsi.router_scores(x, wq, k16), x, ds)
+    at = torch.arange(8 * D, device="cuda")
+    ref = gradient(x, x, wq, k16, ds)[0]
+    q = wq.double().t().repeat(8, 1)
+    n = q * ((q * q).mean(dim=1, keepdim=True) + EPS).rsqrt()
+    a = ds.double() @ k16.double() / 4
+    dq = (a - n * (a * n).mean(dim=1, keepdim=True)) * (n.norm(dim=1) / q.norm(dim=1))[:, None]
+    err = (dx.double() - ref)[at, at % D].norm()
+    assert float(err) <= 4 * U * float((dq.norm(dim=1) * q.norm(dim=1)).norm()), \
+        float(err / (dq.norm(dim=1) * q.norm(dim=1)).norm() / U)
