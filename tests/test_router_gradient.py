@@ -117,3 +117,16 @@ def test_input_gradient_has_no_part_along_the_query():
     err = (dx.double() - ref)[at, at % D].norm()
     assert float(err) <= 4 * U * float((dq.norm(dim=1) * q.norm(dim=1)).norm()), \
         float(err / (dq.norm(dim=1) * q.norm(dim=1)).norm() / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_key_gradient_over_many_tokens(dtype):
+    """dk's error does not grow with the tokens: its sums leave the tensor cores, which round towards zero, every 8
+    steps (one chain over a CTA's tokens: 100 u here)."""
+    M, D, NB = 1 << 18, 256, 32
+    x, wq, k16, ds = inputs(M, D, NB, dtype, "cuda", seed=220)
+    k16 = k16.requires_grad_()
+    got, = torch.autograd.grad(fsi.router_scores(x, wq, k16), k16, ds)
+    ref = gradient(x, x, wq, k16, ds)[2]
+    assert float((got.double() - ref).norm()) <= budget(D) * float(ref.norm()), float((got.double() - ref).norm() / ref.norm() / U)
