@@ -869,11 +869,18 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
       for (int i = 0; i < 4; ++i) {
         const uint32_t a0 = __byte_perm(w0[i], w1[i], 0x5410), a1 = __byte_perm(w0[i], w1[i], 0x7632);
         const uint32_t a2 = __byte_perm(w2[i], w3[i], 0x5410), a3 = __byte_perm(w2[i], w3[i], 0x7632);
+        float c[2][4];  // of this tile alone: the tensor cores round towards zero, a chain over all tiles would add that up
+        mma_bf16_zero(c[0], a0, a1, a2, a3, dq4[2].x, dq4[2].z);
+        mma_bf16_zero(c[1], a0, a1, a2, a3, dq4[2].y, dq4[2].w);
 #pragma unroll
-        for (int k = kDqPieces - 1; k >= 0; --k) {
-          mma_bf16(acc[i][0], a0, a1, a2, a3, dq4[k].x, dq4[k].z);
-          mma_bf16(acc[i][1], a0, a1, a2, a3, dq4[k].y, dq4[k].w);
+        for (int k = 1; k >= 0; --k) {
+          mma_bf16(c[0], a0, a1, a2, a3, dq4[k].x, dq4[k].z);
+          mma_bf16(c[1], a0, a1, a2, a3, dq4[k].y, dq4[k].w);
         }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += c[j][e];
       }
     }
     __syncwarp();  // the tile is in every lane's registers: its place takes the tile kStages on

@@ -123,10 +123,24 @@ def test_input_gradient_has_no_part_along_the_query():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_key_gradient_over_many_tokens(dtype):
     """dk's error does not grow with the tokens: its sums leave the tensor cores, which round towards zero, every 8
-    steps (one chain over a CTA's tokens: 100 u here)."""
+    steps (one chain over a CTA's tokens left 100 u here)."""
     M, D, NB = 1 << 18, 256, 32
     x, wq, k16, ds = inputs(M, D, NB, dtype, "cuda", seed=220)
     k16 = k16.requires_grad_()
     got, = torch.autograd.grad(fsi.router_scores(x, wq, k16), k16, ds)
     ref = gradient(x, x, wq, k16, ds)[2]
+    assert float((got.double() - ref).norm()) <= budget(D) * float(ref.norm()), float((got.double() - ref).norm() / ref.norm() / U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+def test_projection_gradient_over_many_tokens(checkpoint):
+    """dwq's error does not grow with the tokens: a tile of 16 leaves the tensor cores before the next (a chain over
+    a warp's 228 tiles, which round towards zero, left 150 u here)."""
+    M, D, NB = 1 << 17, 4096, 8
+    x, wq, k16, ds = inputs(M, D, NB, torch.bfloat16, "cuda", seed=230)
+    wq = wq.requires_grad_()
+    got, = torch.autograd.grad(fsi.router_scores(x, wq, k16, checkpoint=checkpoint), wq, ds)
+    xk = kept(x, checkpoint)
+    ref = sum(gradient(*(t[a:a + 16384] for t in (x, xk)), wq, k16, ds[a:a + 16384])[1] for a in range(0, M, 16384))
     assert float((got.double() - ref).norm()) <= budget(D) * float(ref.norm()), float((got.double() - ref).norm() / ref.norm() / U)
