@@ -119,7 +119,8 @@ class _PooledTrain(torch.autograd.Function):
         dsoft = dctx @ k16f.t()
         dS = soft * (dsoft - (dsoft * soft).sum(dim=-1, keepdim=True)) / T
         if router:
-            dx_r, dwq, dk16_r = kernels.router_scores_bwd(dS, None, buf, wq.detach(), k16.detach(), *router, dt)
+            # in fp32, whatever the module's type: the parts are summed before they are rounded
+            dx_r, dwq, dk16_r = kernels.router_scores_bwd(dS, None, buf, wq.detach().float(), k16f, *router, torch.float32)
             return (None, dx.add_(dx_r).to(dt), dkg, dku, dv, dwq.to(wq.dtype), (dk16 + dk16_r).to(k16.dtype),
                     dwout.to(wout.dtype))
         xf, wqf = x.float(), wq.detach().float()
