@@ -29,7 +29,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import kernels
-from .training import balance_loss, check_checkpoint, router_scores
+from .training import balance_loss, check_checkpoint, once, router_scores
 
 
 def _chunk_plan(M: int, ch: int) -> list:
@@ -91,6 +91,7 @@ class _PooledTrain(torch.autograd.Function):
         return y, scores, active
 
     @staticmethod
+    @once
     def backward(ctx, dy, _dscores, _dactive):
         x, kg, ku, v, wq, k16, wout, S, active, *router = ctx.saved_tensors
         T, bs = ctx.temperature, ctx.block_size

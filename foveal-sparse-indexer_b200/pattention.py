@@ -45,6 +45,7 @@ class TritonFusedSwiGLUFunction(torch.autograd.Function):
         return kernels.swiglu_fwd(g, u)
 
     @staticmethod
+    @once
     def backward(ctx, dh):
         g, u = ctx.saved_tensors
         dg, du, _ = kernels.swiglu_bwd(dh, g, u, want_h=False)

@@ -69,12 +69,16 @@ def checkpoint_mxfp8(x: Tensor) -> MXFP8Checkpoint:
 
 
 def once(backward):
-    """``once_differentiable`` where the caller builds a graph of the backward pass (a second derivative then
-    raises), the plain function otherwise: the wrapper costs a tenth of a small backward pass."""
-    guarded = once_differentiable(backward)
+    """``once_differentiable`` where the caller builds a graph of the backward pass, the plain function otherwise (the
+    wrapper costs a tenth of a small backward pass).  A second derivative then raises, also where the upstream
+    gradient is a constant (``y.sum()``): the gradients still depend on the saved tensors, so the wrapper is given
+    an argument that requires a gradient."""
+    guarded = once_differentiable(lambda ctx, anchor, *grads: backward(ctx, *grads))
 
     def run(ctx, *grads):
-        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        return guarded(ctx, torch.empty(0, requires_grad=True), *grads)
 
     return run
 

@@ -68,3 +68,60 @@ def test_module_sums_round_once(checkpoint):
     assert 0.5 < float(dx_r.norm() / x0.grad.double().norm()) < 5
     check_rounded_once(xin.grad, x0.grad.double() + dx_r, e)
     check_rounded_once(m.block_keys_16d.grad, dk, e)
+
+
+# ------------------------------------------------------------------ second derivatives
+class Square(torch.autograd.Function):
+    """x^2 whose backward pass saves x and is declared first order."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(x)
+        return x * x
+
+    @staticmethod
+    @fsi.training.once
+    def backward(ctx, d):
+        x, = ctx.saved_tensors
+        return 2 * x.detach() * d
+
+
+def check_first_order(f, leaves, up=None):
+    """The gradients of ``f(*leaves)`` under create_graph are the plain ones, and a penalty on one of them raises
+    instead of losing its own gradient, whether or not the upstream gradient requires one."""
+    plain = torch.autograd.grad(f(*leaves).sum(), leaves)
+    for y_of in (lambda y: y.sum(), lambda y: (y * y).sum()):
+        y = f(*leaves)
+        grads = torch.autograd.grad(y_of(y), leaves, create_graph=True)
+        if y_of(torch.full((2,), 3.0)) == 6.0:
+            assert all(torch.equal(a.detach(), b) for a, b in zip(grads, plain))
+        for g in grads:
+            with pytest.raises(RuntimeError):
+                (y.float().sum() + g.float().pow(2).sum()).backward(retain_graph=True)
+
+
+def test_once_refuses_a_second_derivative():
+    check_first_order(Square.apply, [torch.randn(5, requires_grad=True)])
+    x = torch.randn(5, requires_grad=True)
+    Square.apply(x).sum().backward()
+    assert torch.equal(x.grad, 2 * x.detach()) and not x.grad.requires_grad
+    x.grad = None
+    Square.apply(x).sum().backward(create_graph=True)  # and an in-place update of what it left
+    x.grad.detach_().add_(1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+def test_second_derivatives_raise(checkpoint):
+    x, wq, k16 = (randn(*s, seed=310 + i).requires_grad_() for i, s in enumerate(((40, 64), (16, 64), (8, 16))))
+    check_first_order(lambda *t: fsi.router_scores(*t, checkpoint=checkpoint), [x, wq, k16])
+    g, u = (randn(33, 65, seed=320 + i).requires_grad_() for i in range(2))
+    check_first_order(lambda *t: fsi.triton_fused_swiglu(*t, checkpoint=checkpoint), [g, u])
+    m = make_mlp(torch.float32, checkpoint)
+    xm = randn(20, 256, seed=330).requires_grad_()
+    check_first_order(lambda t, *_: m(t), [xm, m.q_proj_16d.weight, m.block_keys_16d, m.out_proj_16d.weight, m.v])
+    check_first_order(lambda t, *_: m.balance_loss(t)[0], [xm, m.q_proj_16d.weight, m.block_keys_16d])
+    s = randn(50, 8, seed=340).requires_grad_()
+    idx = torch.full((50, 1), 5, dtype=torch.int32, device="cuda")
+    cnt = torch.ones(50, dtype=torch.int32, device="cuda")
+    check_first_order(lambda t: fsi.balance_loss(t, idx, cnt, base_blocks=1)[0], [s])
