@@ -29,7 +29,7 @@ import torch.nn.functional as F
 from torch import Tensor, nn
 
 from . import kernels
-from .training import balance_loss, check_checkpoint, once, router_scores
+from .training import balance_loss, check_checkpoint, check_router, checked_balance, once, router_scores
 
 
 def _chunk_plan(M: int, ch: int) -> list:
@@ -134,6 +134,47 @@ class _PooledTrain(torch.autograd.Function):
         dwq = dq.t() @ xf
         dx = dx + dq @ wqf
         return (None, dx.to(dt), dkg, dku, dv, dwq.to(wq.dtype), dk16.to(k16.dtype), dwout.to(wout.dtype))
+
+
+class _KeptBalance(torch.autograd.Function):
+    """``FovealPattentionMLP.balance_loss`` of a module with a checkpoint, which keeps neither x nor a copy of it.
+
+    x enters the gradients of q_proj and block_keys only, and the loss's upstream gradient is one number: both are
+    computed in the forward for the upstream gradient 1 (fp32, 16 (D + NB) numbers) and scaled in the backward.
+    dx = dq q_proj takes the scores (4 NB bytes a token) and the queries (68)."""
+
+    @staticmethod
+    def forward(ctx, module, x, wq, k16, valid):
+        base, T = module.base_blocks, module.temperature
+        scores, saved, _ = kernels.router_scores_train(x, wq, k16)
+        loss, counts, state = checked_balance(scores, *module._token_routes(scores), base, T, valid)
+        _, need_x, need_w, need_k, _ = ctx.needs_input_grad
+        dw = dk = None
+        if need_w or need_k:
+            one = torch.ones((), dtype=torch.float32, device=scores.device)
+            ds = kernels.balance_loss_bwd(scores, base, T, valid, state, one)
+            _, dw, dk = kernels.router_scores_bwd(ds, x, None, wq.float(), k16.float(), saved, x.dtype,
+                                                  (False, need_w, need_k))
+        kept = (scores, saved, valid, state, wq, k16) if need_x else (None,) * 6
+        ctx.save_for_backward(*kept, dw, dk)
+        ctx.base, ctx.temperature, ctx.dtypes = base, T, (x.dtype, wq.dtype, k16.dtype)
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return loss, counts
+
+    @staticmethod
+    @once
+    def backward(ctx, dloss, _dcounts):
+        if dloss is None:
+            return (None,) * 5
+        scores, saved, valid, state, wq, k16, dw, dk = ctx.saved_tensors
+        dx = None
+        if scores is not None:
+            ds = kernels.balance_loss_bwd(scores, ctx.base, ctx.temperature, valid, state, dloss)
+            dx, _, _ = kernels.router_scores_bwd(ds, None, None, wq, k16, saved, ctx.dtypes[0], (True, False, False))
+        dw = (dw * dloss).to(ctx.dtypes[1]) if dw is not None else None
+        dk = (dk * dloss).to(ctx.dtypes[2]) if dk is not None else None
+        return None, dx, dw, dk, None
 
 
 class _ForwardOnly(torch.autograd.Function):
@@ -333,11 +374,21 @@ class FovealPattentionMLP(nn.Module):
         The routes are the ones ``routing="token"`` takes (``top_p``, ``min_remote_blocks``,
         ``max_remote_blocks``); the loss reaches x, q_proj_16d and block_keys_16d through the router scores.
         ``valid`` (bool [...]) leaves out padding, whose rows of x have to be finite all the same where a
-        gradient is taken (0 times NaN is NaN in the router's own backward pass).  Add a small multiple to the training loss to keep the
-        blocks' loads even; see :func:`training.balance_loss`."""
+        gradient is taken (0 times NaN is NaN in the router's own backward pass).  Add a small multiple to the
+        training loss to keep the blocks' loads even; see :func:`training.balance_loss`.  With a ``checkpoint``
+        nothing of x's size is kept for the backward pass."""
         xx = x.to(self.k_gate.dtype)
-        scores = router_scores(xx, self.q_proj_16d.weight, self.block_keys_16d, checkpoint=self.checkpoint)
-        s2d = scores.detach().reshape(-1, self.num_blocks)
+        wq, k16 = self.q_proj_16d.weight, self.block_keys_16d
+        if check_checkpoint(self.checkpoint) is not None and torch.is_grad_enabled():
+            check_router(xx, wq, k16)
+            return _KeptBalance.apply(self, xx, wq, k16, valid)
+        scores = router_scores(xx, wq, k16)
+        idx, cnt = self._token_routes(scores.detach())
+        return balance_loss(scores, idx, cnt, base_blocks=self.base_blocks, temperature=self.temperature, valid=valid)
+
+    def _token_routes(self, scores: Tensor) -> Tuple[Tensor, Tensor]:
+        """(remote_indices [..., capacity], remote_counts [...]) that token routing selects from ``scores`` [..., NB]."""
+        lead, s2d = scores.shape[:-1], scores.reshape(-1, self.num_blocks)
         cap = max(int(self.max_remote_blocks), 1)
         if s2d.numel() == 0:  # no tokens: nothing to select from
             idx, cnt = (torch.empty(n, dtype=torch.int32, device=s2d.device) for n in ((0, cap), (0,)))
@@ -346,9 +397,7 @@ class FovealPattentionMLP(nn.Module):
                 idx, cnt, _, _ = kernels.select(s2d, base_blocks=self.base_blocks, top_p=self.top_p,
                                                 min_remote=self.min_remote_blocks, max_remote=self.max_remote_blocks,
                                                 capacity=cap, temperature=self.temperature)
-        lead = x.shape[:-1]
-        return balance_loss(scores, idx.view(*lead, cap), cnt.view(lead), base_blocks=self.base_blocks,
-                            temperature=self.temperature, valid=valid)
+        return idx.view(*lead, cap), cnt.view(lead)
 
     # ------------------------------------------------------------------ helpers
     def _packed(self):

@@ -101,11 +101,8 @@ class _RouterScores(torch.autograd.Function):
         return dx, dw, dk, None
 
 
-def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: Optional[str] = None) -> Tensor:
-    """``rms_norm(x q_proj^T) block_keys^T / 4`` per token, differentiable in all three: x [..., D] fp32 or
-    bf16, q_proj [16, D], block_keys [NB, 16] -> fp32 [..., NB].  With ``checkpoint="mxfp8"`` the backward
-    pass reads an 8-bit copy of x (it enters q_proj's gradient only)."""
-    check_checkpoint(checkpoint)
+def check_router(x: Tensor, q_proj: Tensor, block_keys: Tensor) -> None:
+    """Refuses what :func:`router_scores` does not take."""
     for t in (x, q_proj, block_keys):
         dtype_code(t.dtype)
     D = x.shape[-1] if x.dim() else 0
@@ -116,6 +113,14 @@ def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: 
     NB = block_keys.shape[0]
     if D == 0 or D % 8 or not 1 <= NB <= 1024:
         raise ValueError(f"the router takes widths that are multiples of 8 and 1 to 1024 blocks, got D {D}, NB {NB}")
+
+
+def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: Optional[str] = None) -> Tensor:
+    """``rms_norm(x q_proj^T) block_keys^T / 4`` per token, differentiable in all three: x [..., D] fp32 or
+    bf16, q_proj [16, D], block_keys [NB, 16] -> fp32 [..., NB].  With ``checkpoint="mxfp8"`` the backward
+    pass reads an 8-bit copy of x (it enters q_proj's gradient only)."""
+    check_checkpoint(checkpoint)
+    check_router(x, q_proj, block_keys)
     grad = torch.is_grad_enabled() and (x.requires_grad or q_proj.requires_grad or block_keys.requires_grad)
     return _RouterScores.apply(x, q_proj, block_keys, grad and checkpoint is not None)
 
@@ -175,21 +180,8 @@ class _BalanceLoss(torch.autograd.Function):
         return ds, None, None, None, None, None, None
 
 
-def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts: Optional[Tensor], *,
-                 base_blocks: int, temperature: float = 1.0, valid: Optional[Tensor] = None,
-                 counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
-    """Load-balance loss of a routing and the blocks' slot counts.
-
-    scores [..., NB] are the router's scores (before the temperature), remote_indices [..., capacity] and
-    remote_counts [...] the routes chosen from them (``select_blocks``).  With p_t the softmax of
-    scores_t / temperature over the R = NB - base_blocks remote blocks, f_b block b's share of the slots and n
-    the number of rows, ``loss = R sum_b f_b (1/n) sum_t p_tb``: 1 for an even load, R when one block takes
-    everything.  Temperatures from 1e-30 to 1e30, at most 2^20 slots to a list.  The gradient reaches the scores through p only.
-
-    Rows whose ``valid`` is False or whose remote scores are all -inf are not counted in n and receive zeros;
-    the slots are those of :func:`block_counts`, which leaves out the rows whose ``valid`` is False only.
-    ``counts`` (int64 [NB], :func:`block_counts` summed over ranks) replaces the lists' own counts; the
-    lists may be None then.  Returns (loss fp32 0-d, counts int64 [NB])."""
+def _check_balance(scores, remote_indices, remote_counts, base_blocks, temperature, valid, counts=None):
+    """The arguments of :func:`balance_loss`, refused or in the kernels' types."""
     NB = _check_blocks(scores.shape[-1] if scores.dim() else 0)
     if not 0 <= int(base_blocks) < NB:
         raise ValueError(f"base_blocks must leave a remote block: 0 <= base_blocks < {NB}, got {base_blocks}")
@@ -212,4 +204,31 @@ def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts
     _check_valid(valid, lead)
     if scores.dtype != torch.float32:
         scores = scores.float()
-    return _BalanceLoss.apply(scores, remote_indices, remote_counts, int(base_blocks), float(temperature), valid, counts)
+    return scores, remote_indices, remote_counts, int(base_blocks), float(temperature)
+
+
+def checked_balance(scores: Tensor, remote_indices: Tensor, remote_counts: Tensor, base_blocks: int,
+                    temperature: float, valid: Optional[Tensor]):
+    """(loss, counts, state) of :func:`balance_loss`'s forward, without a graph."""
+    scores, idx, cnt, base, T = _check_balance(scores, remote_indices, remote_counts, base_blocks, temperature, valid)
+    return kernels.balance_loss_fwd(scores, idx, cnt, scores.shape[-1], base, T, valid)
+
+
+def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts: Optional[Tensor], *,
+                 base_blocks: int, temperature: float = 1.0, valid: Optional[Tensor] = None,
+                 counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Load-balance loss of a routing and the blocks' slot counts.
+
+    scores [..., NB] are the router's scores (before the temperature), remote_indices [..., capacity] and
+    remote_counts [...] the routes chosen from them (``select_blocks``).  With p_t the softmax of
+    scores_t / temperature over the R = NB - base_blocks remote blocks, f_b block b's share of the slots and n
+    the number of rows, ``loss = R sum_b f_b (1/n) sum_t p_tb``: 1 for an even load, R when one block takes
+    everything.  Temperatures from 1e-30 to 1e30, at most 2^20 slots to a list.  The gradient reaches the scores through p only.
+
+    Rows whose ``valid`` is False or whose remote scores are all -inf are not counted in n and receive zeros;
+    the slots are those of :func:`block_counts`, which leaves out the rows whose ``valid`` is False only.
+    ``counts`` (int64 [NB], :func:`block_counts` summed over ranks) replaces the lists' own counts; the
+    lists may be None then.  Returns (loss fp32 0-d, counts int64 [NB])."""
+    scores, idx, cnt, base, T = _check_balance(scores, remote_indices, remote_counts, base_blocks, temperature, valid,
+                                               counts)
+    return _BalanceLoss.apply(scores, idx, cnt, base, T, valid, counts)

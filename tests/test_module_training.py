@@ -125,3 +125,92 @@ def test_second_derivatives_raise(checkpoint):
     idx = torch.full((50, 1), 5, dtype=torch.int32, device="cuda")
     cnt = torch.ones(50, dtype=torch.int32, device="cuda")
     check_first_order(lambda t: fsi.balance_loss(t, idx, cnt, base_blocks=1)[0], [s])
+
+
+# ------------------------------------------------------------------ the balance loss of a module with a checkpoint
+def balance_gradients(m, x, valid):
+    """(loss, dx, dwq, dk) of the module's balance loss in 64 bits, on the routes that token routing takes."""
+    base, T = m.base_blocks, m.temperature
+    s, idx, cnt = None, None, None
+    with torch.no_grad():
+        s = m.compute_router_scores(x)
+        idx, cnt, _, _ = kernels.select(s, base_blocks=base, top_p=m.top_p, min_remote=m.min_remote_blocks,
+                                        max_remote=m.max_remote_blocks, capacity=m.max_remote_blocks, temperature=T)
+    live = (torch.arange(idx.shape[1], device=x.device) < cnt[:, None]) & valid[:, None]
+    counts = torch.bincount(idx[live].long(), minlength=m.num_blocks)
+    leaves = [t.detach().double().requires_grad_() for t in (x, m.q_proj_16d.weight, m.block_keys_16d)]
+    xx, wq, k16 = leaves
+    q = xx @ wq.t()
+    n = q * ((q * q).mean(dim=1, keepdim=True) + EPS).rsqrt()
+    p = torch.softmax((n @ k16.t() / 4)[:, base:] / T, dim=1)[valid]
+    f = counts[base:].double() / int(counts.sum())
+    loss = (m.num_blocks - base) * (f * p.mean(dim=0)).sum()
+    return (loss.detach(), counts, *torch.autograd.grad(loss, leaves))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lead,D", [((3, 70), 256), ((401,), 1000)])
+def test_balance_loss_of_a_checkpointed_module(lead, D, dtype):
+    """The loss and counts are those without a checkpoint; the gradients, under an upstream gradient of 0.3 and for each
+    subset of what requires one, are the 64-bit formula's, rounded once (e: the router gradient's budget, and as
+    much for the softmax and its projection)."""
+    m, plain = make_mlp(dtype, "mxfp8", D=D), make_mlp(dtype, None, D=D)
+    x = randn(*lead, D, seed=350, dtype=dtype)
+    valid = torch.rand(lead, generator=torch.Generator(device="cuda").manual_seed(351), device="cuda") < 0.8
+    loss, counts, *ref = balance_gradients(m, x.reshape(-1, D), valid.reshape(-1))
+    e = 2 * budget(D)
+    full = None
+    for mask in (7, 1, 2, 4, 6):
+        xin = x.clone().requires_grad_(bool(mask & 1))
+        leaves = [xin, m.q_proj_16d.weight.requires_grad_(bool(mask & 2)), m.block_keys_16d.requires_grad_(bool(mask & 4))]
+        got, c = m.balance_loss(xin, valid)
+        pl, pc = plain.balance_loss(x, valid)
+        assert torch.equal(got.detach(), pl.detach()) and torch.equal(c, pc) and torch.equal(c, counts)
+        assert abs(float(got.detach()) - float(loss)) <= e * float(loss)
+        want = [i for i in range(3) if mask >> i & 1]
+        grads = torch.autograd.grad(got, [leaves[i] for i in want], torch.full((), 0.3, device="cuda"))
+        if mask == 7:
+            full = grads
+            for g, r in zip(grads, ref):
+                g, r = g.reshape(r.shape), 0.3 * r
+                if dtype == torch.bfloat16:
+                    check_rounded_once(g, r, e)
+                else:
+                    assert float((g.double() - r).norm()) <= e * float(r.norm())
+            assert not bool(grads[0][~valid].any())
+        assert all(torch.equal(g, full[i]) for g, i in zip(grads, want))
+    with torch.no_grad():
+        assert m.balance_loss(x, valid)[0].grad_fn is None
+    with pytest.raises(ValueError):
+        m.balance_loss(x[..., :D - 8])
+    y = torch.zeros(0, D, dtype=dtype, device="cuda", requires_grad=True)
+    g = torch.autograd.grad(m.requires_grad_().balance_loss(y)[0], [y, m.q_proj_16d.weight, m.block_keys_16d])
+    assert g[0].shape == (0, D) and not bool(g[1].any()) and not bool(g[2].any())
+
+
+def held_bytes(checkpoint, M, D):
+    """Bytes that a step's graph holds between the passes, with x itself an activation that only the graph keeps."""
+    m = make_mlp(torch.bfloat16, checkpoint, D=D)
+    leaf = randn(M, D, seed=360, dtype=torch.bfloat16).requires_grad_()
+    for _ in range(2):  # the first step leaves packed weights and workspaces
+        m.zero_grad(set_to_none=True)
+        leaf.grad = None
+        before = torch.cuda.memory_allocated()
+        x = leaf * 1.0
+        y, (loss, counts) = m(x), m.balance_loss(x)
+        del x
+        held = torch.cuda.memory_allocated() - before - y.numel() * 2
+        torch.autograd.backward([y, loss], [torch.ones_like(y), torch.ones_like(loss)])
+        del y, loss, counts
+    return held
+
+
+@pytest.mark.gpu
+def test_step_with_a_checkpoint_holds_fewer_bytes():
+    """Output and balance loss of one step: without a checkpoint both keep x (2 bytes an element, once), with it one
+    8-bit copy (1 + 1/32) is left.  Queries (68 bytes a token), q_proj's gradient (64 D bytes) and rounded
+    allocations are the rest: 0.88 bytes an element fewer at 1024 wide."""
+    M, D = 8192, 1024
+    plain, kept = held_bytes(None, M, D), held_bytes("mxfp8", M, D)
+    assert 2 * M * D <= plain and kept <= plain - 0.88 * M * D, (plain / M / D, kept / M / D)
