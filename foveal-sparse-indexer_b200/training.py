@@ -87,15 +87,14 @@ class _RouterScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, q_proj, block_keys, keep):
         scores, saved, buf = kernels.router_scores_train(x, q_proj, block_keys, keep_mxfp8=keep)
-        ctx.keep, ctx.dtype = keep, x.dtype
-        ctx.save_for_backward(buf if keep else x, q_proj, block_keys, saved)
+        ctx.dtype = x.dtype
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] and not keep else None, buf, q_proj, block_keys, saved)
         return scores
 
     @staticmethod
     @once
     def backward(ctx, dscores):
-        kept, q_proj, block_keys, saved = ctx.saved_tensors
-        x, buf = (None, kept) if ctx.keep else (kept, None)
+        x, buf, q_proj, block_keys, saved = ctx.saved_tensors
         dx, dw, dk = kernels.router_scores_bwd(dscores, x, buf, q_proj, block_keys, saved, ctx.dtype,
                                                ctx.needs_input_grad)
         return dx, dw, dk, None
@@ -121,8 +120,9 @@ def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: 
     pass reads an 8-bit copy of x (it enters q_proj's gradient only)."""
     check_checkpoint(checkpoint)
     check_router(x, q_proj, block_keys)
-    grad = torch.is_grad_enabled() and (x.requires_grad or q_proj.requires_grad or block_keys.requires_grad)
-    return _RouterScores.apply(x, q_proj, block_keys, grad and checkpoint is not None)
+    # only q_proj's gradient reads the tokens: without it neither x nor a copy is kept
+    keep = checkpoint is not None and torch.is_grad_enabled() and q_proj.requires_grad
+    return _RouterScores.apply(x, q_proj, block_keys, keep)
 
 
 def _check_routes(remote_indices: Tensor, remote_counts: Tensor) -> None:

@@ -214,3 +214,24 @@ def test_step_with_a_checkpoint_holds_fewer_bytes():
     M, D = 8192, 1024
     plain, kept = held_bytes(None, M, D), held_bytes("mxfp8", M, D)
     assert 2 * M * D <= plain and kept <= plain - 0.88 * M * D, (plain / M / D, kept / M / D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+def test_router_scores_keep_the_tokens_for_q_proj_only(checkpoint, dtype):
+    """Where q_proj takes no gradient (a frozen projection), nothing of x's size is kept, and the other gradients are the
+    same bits."""
+    x, wq, k16 = randn(120, 256, seed=370, dtype=dtype), randn(16, 256, seed=371, dtype=dtype), randn(9, 16, seed=372, dtype=dtype)
+    ds = randn(120, 9, seed=373)
+    leaves = [t.clone().requires_grad_() for t in (x, wq, k16)]
+    full = torch.autograd.grad(fsi.router_scores(*leaves, checkpoint=checkpoint), leaves, ds)
+    for frozen, kept in ((True, 0), (False, 256 + 8 if checkpoint else 256 * x.element_size())):
+        xin, k = x.clone().requires_grad_(), k16.clone().requires_grad_()
+        w = wq.clone().requires_grad_(not frozen)
+        s = fsi.router_scores(xin, w, k, checkpoint=checkpoint)
+        sizes = sorted(t.numel() * t.element_size() for t in s.grad_fn.saved_tensors if t is not None)
+        rest = [w.numel() * w.element_size(), k.numel() * k.element_size(), 17 * 120 * 4]
+        assert sizes == sorted(rest + ([120 * kept] if kept else [])), (frozen, sizes)
+        dx, dk = torch.autograd.grad(s, (xin, k), ds)
+        assert torch.equal(dx, full[0]) and torch.equal(dk, full[2])
