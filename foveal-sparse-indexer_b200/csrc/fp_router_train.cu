@@ -1083,19 +1083,29 @@ sum_partials_kernel(const float* __restrict__ p1, int parts1, int64_t n1, T* __r
 
 // Launch shapes and workspace of the three passes: about two CTAs of pass 2 to an SM (three for fp32), and no
 // more partial sums than that.
+// Rows of codes that TMA cannot address (D % 16 != 0, bf16) go through pass 2 as bf16 in pieces: of 64 MB, which stay
+// in L2 between the two kernels, or of a sixteenth of the rows, an eighth of the codes, where that is more.  Against
+// all rows at once (2 bytes an element of workspace): 65536 x 1000 183 -> 160 us, 65536 x 4104 419 -> 477 us (with
+// pieces of 32 MB 560 us).
+constexpr int64_t kCopyBytes = 64 << 20;
 struct BwdPlan {
-  int dq_ctas, wide, col_ctas, parts;
-  int64_t per_cta;  // pass 2: tiles of 16 tokens (bf16) or tokens (fp32)
+  int dq_ctas, wide, col_ctas, parts, pieces;
+  int64_t per_cta;     // pass 2: tiles of 16 tokens (bf16) or tokens (fp32)
+  int64_t piece_rows;  // M unless the rows go in pieces
   size_t dq, dw, dk, copy, total;
 };
 BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB, bool from_codes) {
   BwdPlan p{};
   p.dq_ctas = (int)std::min<int64_t>((M + kDqTokens - 1) / kDqTokens, kDqMaxCtas);
+  const bool copied = from_codes && dtype == FP_DTYPE_BF16 && D % 16;
+  p.piece_rows = M;
+  if (copied) p.piece_rows = std::min(M, (std::max((kCopyBytes / 2 + D - 1) / D, (M + 15) / 16) + 15) / 16 * 16);
+  p.pieces = (int)((M + p.piece_rows - 1) / p.piece_rows);
   int64_t units;
   if (dtype == FP_DTYPE_BF16) {
     p.wide = D <= 64 ? 1 : D <= 128 ? 2 : 4;
     p.col_ctas = (D + 64 * p.wide - 1) / (64 * p.wide);
-    units = (M + 15) / 16;
+    units = (p.piece_rows + 15) / 16;
     p.per_cta = std::max<int64_t>((units + std::max(296 / p.col_ctas, 1) - 1) / std::max(296 / p.col_ctas, 1),
                                   2 * kXWarps / p.wide);
   } else {
@@ -1109,9 +1119,9 @@ BwdPlan bwd_plan(int dtype, int64_t M, int D, int NB, bool from_codes) {
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   p.dq = 0;
   p.dw = p.dq + up((size_t)((M + 15) / 16) * (dtype == FP_DTYPE_BF16 ? kDqTileBytes : 16 * kIdx * 4));
-  p.dk = p.dw + up((size_t)p.parts * kIdx * D * 4);
+  p.dk = p.dw + up((size_t)p.parts * p.pieces * kIdx * D * 4);
   p.copy = p.dk + up((size_t)p.dq_ctas * kIdx * NB * 4);
-  p.total = p.copy + (from_codes && dtype == FP_DTYPE_BF16 && D % 16 ? up((size_t)M * D * 2) : 0);
+  p.total = p.copy + (copied ? up((size_t)p.piece_rows * D * 2) : 0);
   return p;
 }
 
@@ -1138,41 +1148,52 @@ int router_bwd(const float* ds, const T* x, const uint8_t* codes, const uint8_t*
   if (const int rc = NB % 4 == 0 ? launch_dq<T, true>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st)
                                  : launch_dq<T, false>(p, ds, k16, q16, rnorm, M, NB, dq, pk, st))
     return rc;
+  int parts = p.parts;
   if (dq) {
     const dim3 grid(p.col_ctas, p.parts);
-    cudaError_t e;
     if constexpr (sizeof(T) == 2) {
       static_assert(kXSmem<true> >= kXWarps * 64 * kIdx * 4 + 1024, "the ring's place takes the sums");
-      const __nv_bfloat16* rows = x;
-      if (codes && D % 16) {  // rows of codes that TMA cannot address: as bf16 in the workspace
-        rows = reinterpret_cast<const __nv_bfloat16*>(ws + p.copy);
-        if (dwq)
-          if (const int rc = fp_mxfp8_dequantize(codes, scales, FP_DTYPE_BF16, M * D, ws + p.copy, st)) return rc;
-        codes = nullptr;
+      const bool copied = codes && D % 16;
+      // without dWq nothing reads the rows, and one launch takes them all
+      const int64_t step = copied && dwq ? p.piece_rows : M;
+      const bool from_codes = codes && !copied;
+      const auto kern = from_codes ? router_x_kernel<true> : router_x_kernel<false>;
+      const int smem = from_codes ? kXSmem<true> : kXSmem<false>;
+      if (!(from_codes ? allow_smem<router_x_kernel<true>>(smem) : allow_smem<router_x_kernel<false>>(smem)))
+        return FP_ERR_CUDA;
+      parts = 0;
+      for (int64_t r0 = 0; r0 < M; r0 += step, parts += p.parts) {
+        const int64_t n = std::min(step, M - r0);  // r0 is a multiple of 16 tokens, r0 D one of 128 elements
+        const __nv_bfloat16* rows = x;
+        if (copied && dwq) {
+          rows = reinterpret_cast<const __nv_bfloat16*>(ws + p.copy);
+          if (const int rc = fp_mxfp8_dequantize(codes + r0 * D, scales + r0 * D / kMxBlock, FP_DTYPE_BF16, n * D,
+                                                 ws + p.copy, st))
+            return rc;
+        }
+        CUtensorMap map{};
+        if (dwq && !(from_codes ? encode_map_2d_u8(&map, codes, D, n, D, 64, 16)
+                                : encode_map_2d(&map, rows, D, n, (uint64_t)D * 2, 64, 16)))
+          return FP_ERR_CUDA;
+        const uint4* dqt = reinterpret_cast<const uint4*>((const char*)dq + r0 / 16 * kDqTileBytes);
+        if (launch_pdl(kern, grid, kXWarps * 32, smem, st, map, scales, dqt, wq, n, D, p.wide,
+                       dx ? dx + r0 * D : nullptr, pw ? pw + (int64_t)parts * kIdx * D : nullptr) != cudaSuccess)
+          return FP_ERR_CUDA;
       }
-      const auto kern = codes ? router_x_kernel<true> : router_x_kernel<false>;
-      const int smem = codes ? kXSmem<true> : kXSmem<false>;
-      CUtensorMap map{};
-      if (dwq && !(codes ? encode_map_2d_u8(&map, codes, D, M, D, 64, 16)
-                         : encode_map_2d(&map, rows, D, M, (uint64_t)D * 2, 64, 16)))
-        return FP_ERR_CUDA;
-      if (!(codes ? allow_smem<router_x_kernel<true>>(smem) : allow_smem<router_x_kernel<false>>(smem)))
-        return FP_ERR_CUDA;
-      e = launch_pdl(kern, grid, kXWarps * 32, smem, st, map, scales, (const uint4*)dq, wq, M, D, p.wide, dx, pw);
-    } else
-      e = launch_pdl(codes ? router_x_f32_kernel<true> : router_x_f32_kernel<false>, grid, kFThreads, 0, st, x, codes,
-                     scales, (const float*)dq, wq, M, D, p.wide, p.per_cta, dx, pw);
-    if (e != cudaSuccess) return FP_ERR_CUDA;
+    } else if (launch_pdl(codes ? router_x_f32_kernel<true> : router_x_f32_kernel<false>, grid, kFThreads, 0, st, x,
+                          codes, scales, (const float*)dq, wq, M, D, p.wide, p.per_cta, dx, pw) != cudaSuccess) {
+      return FP_ERR_CUDA;
+    }
   }
   if (dwq || dk16) {
     const int64_t n1 = dwq ? (int64_t)kIdx * D : 0, n2 = dk16 ? (int64_t)kIdx * NB : 0;
     const unsigned grid = (unsigned)((n1 + 31) / 32 + (n2 + 31) / 32);
     cudaError_t e;
     if (grad_dtype == FP_DTYPE_BF16)
-      e = launch_pdl(sum_partials_kernel<__nv_bfloat16>, grid, 256, 0, st, pw, p.parts, n1, (__nv_bfloat16*)dwq, pk,
+      e = launch_pdl(sum_partials_kernel<__nv_bfloat16>, grid, 256, 0, st, pw, parts, n1, (__nv_bfloat16*)dwq, pk,
                      p.dq_ctas, n2, (__nv_bfloat16*)dk16);
     else
-      e = launch_pdl(sum_partials_kernel<float>, grid, 256, 0, st, pw, p.parts, n1, (float*)dwq, pk, p.dq_ctas, n2,
+      e = launch_pdl(sum_partials_kernel<float>, grid, 256, 0, st, pw, parts, n1, (float*)dwq, pk, p.dq_ctas, n2,
                      (float*)dk16);
     if (e != cudaSuccess) return FP_ERR_CUDA;
   }

@@ -58,7 +58,7 @@ def gradient(x, xq, wq, k16, ds):
 def check_norms(got, ref, dtype, e):
     """dx, dwq and dk as wholes, and dwq by router dimension, dx by token and dk by block: none may have less
     than the average of the allowance."""
-    for name, g, r in zip(("dx", "dwq", "dk"), got, ref):
+    for name, g, r in zip(("dx", "dwq", "dk")[-len(got):], got, ref):
         assert bool(torch.isfinite(g).all()), name
         one = r.double()
         tol = e
@@ -144,3 +144,33 @@ def test_projection_gradient_over_many_tokens(checkpoint):
     xk = kept(x, checkpoint)
     ref = sum(gradient(*(t[a:a + 16384] for t in (x, xk)), wq, k16, ds[a:a + 16384])[1] for a in range(0, M, 16384))
     assert float((got.double() - ref).norm()) <= budget(D) * float(ref.norm()), float((got.double() - ref).norm() / ref.norm() / U)
+
+
+# Widths whose rows of codes TMA cannot address: they go through the workspace as bf16, in pieces.
+PIECES = [(40000, 1000, 24), (33568, 1000, 5), (33569, 1000, 5), (4200000, 8, 3)]
+
+
+def test_workspace_of_unaligned_codes_stays_small():
+    """A piece is at most 64 MB or an eighth of the codes (a sixteenth of the rows in bf16), not all of x in bf16."""
+    __import__("importlib").import_module("foveal-sparse-indexer_b200.build").build()
+    size = fsi.load_library().fp_router_scores_bwd_workspace_size
+    for M, D in [(4096, 1000), (131072, 1000), (1 << 20, 1000), (1 << 20, 4104), (1 << 22, 8), (1 << 27, 8)]:
+        codes, extra = M * D, size(1, M, D, 64, 1) - size(1, M, D, 64, 0)
+        # and a set of partial sums of dwq a piece: 296 CTAs, 256 columns each, 16 sums of 4 bytes a column
+        pieces = min(16, -(-codes // (32 << 20))) + 1
+        assert 0 < extra <= max((64 << 20) + 512 * D, codes // 8 + 512 * D) + pieces * 296 * 256 * 64, (M, D, extra)
+        assert size(1, M, D + 8, 64, 1) - size(1, M, D + 8, 64, 0) == 0  # addressable rows need none
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,D,NB", PIECES)
+def test_gradient_from_unaligned_codes_in_pieces(M, D, NB):
+    """More than one piece, and last pieces of one row, of a part of a tile and of all rows: dx is that of the uncopied
+    input bit by bit, dwq and dk are the 64-bit formula's at the copy."""
+    x, wq, k16, ds = inputs(M, D, NB, torch.bfloat16, "cuda", seed=240)
+    got, plain = run(x, wq, k16, ds, "mxfp8"), run(x, wq, k16, ds, None)
+    assert torch.equal(got[0], plain[0])
+    check_norms(got[1:], gradient(x, kept(x, True), wq, k16, ds)[1:], torch.float32, budget(D))
+    part = [t.clone().requires_grad_(i != 1) for i, t in enumerate((x, wq, k16))]  # no gradient for q_proj: one launch
+    dx, = torch.autograd.grad(fsi.router_scores(*part, checkpoint="mxfp8"), part[0], ds)
+    assert torch.equal(dx, got[0])
