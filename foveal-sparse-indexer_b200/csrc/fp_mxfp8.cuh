@@ -196,6 +196,4 @@ struct MxVec {
   }
 };
 
-__device__ __forceinline__ float mx_value(uint8_t code, int byte) { return mx_unpack2(code).x * mx_scale(byte); }
-
 }  // namespace fp
