@@ -30,6 +30,7 @@ U = 2.0 ** -24
 EPS = 1.1920928955078125e-07
 SIZES = [(1, 8, 1), (1, 64, 16), (3, 72, 5), (16, 256, 16), (17, 264, 33), (64, 256, 224), (130, 1000, 65),
          (33, 512, 1024), (257, 1024, 130), (1000, 128, 12), (700, 512, 448)]
+LARGE = [(2111, 4096, 224), (5000, 2056, 64), (9001, 1536, 1000)]  # many CTAs along both sides, odd ends
 
 
 def budget(D):
@@ -87,13 +88,61 @@ def kept(x, checkpoint):
 @pytest.mark.gpu
 @pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("M,D,NB", SIZES)
+@pytest.mark.parametrize("M,D,NB", SIZES + LARGE)
 def test_gradient_norms(M, D, NB, dtype, checkpoint):
     x, wq, k16, ds = inputs(M, D, NB, dtype, "cuda")
     got = run(x, wq, k16, ds, checkpoint)
     assert [g.dtype for g in got] == [dtype, torch.float32, torch.float32]
     check_norms(got, gradient(x, kept(x, checkpoint), wq, k16, ds), dtype, budget(D))
 
+
+
+def pieces(v, k):
+    """``v`` as the sum of its k leading bf16 pieces."""
+    out = torch.zeros_like(v)
+    for _ in range(k):
+        out = out + (v - out).to(torch.bfloat16).double()
+    return out
+
+
+def mutants(x, wq, k16, ds):
+    """(name, gradients) of calculations that are wrong or too coarse."""
+    x, wq, k16, ds = (t.double() for t in (x, wq, k16, ds))
+    q = x @ wq.t()
+    r = ((q * q).mean(dim=1, keepdim=True) + EPS).rsqrt()
+    n = q * r
+    a = ds @ k16 / 4
+    dq = r * (a - n * (a * n).mean(dim=1, keepdim=True))
+    dk = ds.t() @ n / 4
+    right = (dq @ wq, dq.t() @ x, dk)
+    for i, name in enumerate(("dx", "dwq", "dk")):
+        yield name + " zero", tuple(torch.zeros_like(t) if i == j else t for j, t in enumerate(right))
+        yield name + " of one token less", tuple(
+            (torch.cat([t[:-1], 0 * t[-1:]]) if i == 0 else t - (dq[-1:].t() @ x[-1:] if i == 1 else ds[-1:].t() @ n[-1:] / 4))
+            if i == j else t for j, t in enumerate(right))
+    for name, d in (("no projection", r * a), ("no factor", dq / r), ("dq in one bf16 piece", pieces(dq, 1))):
+        yield name + " in dx", (d @ wq, right[1], dk)
+        yield name + " in dwq", (right[0], d.t() @ x, dk)
+    yield "a transposed sign", (right[0], right[1], -dk)
+    if x.shape[0] >= 16:  # (a few elements alone may be rounded well by chance)
+        yield "dq in two bf16 pieces", (right[0], pieces(dq, 2).t() @ x, dk)
+        yield "dk off by 2^-12", (right[0], right[1], dk * (1 + 2.0 ** -12))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,D,NB", SIZES)
+def test_the_norms_reject_what_is_wrong(M, D, NB, dtype):
+    """On the CPU, at every size: the right gradients pass, rounded to the outputs' types, and every wrong one fails."""
+    x, wq, k16, ds = inputs(M, D, NB, dtype, "cpu")
+    ref = gradient(x, x, wq, k16, ds)
+    out = lambda t: (t[0].to(dtype), t[1].float(), t[2].float())
+    check_norms(out(ref), ref, dtype, budget(D))
+    for name, t in mutants(x, wq, k16, ds):
+        if dtype == torch.bfloat16 and name == "dq in one bf16 piece in dx" and M * D < 4096:
+            continue  # bf16 outputs of few elements: the allowance for the chance in their rounding is as large
+        with pytest.raises(AssertionError):
+            check_norms(out(t), ref, dtype, budget(D))
+            raise ValueError(f"not rejected: {name}")
 
 @pytest.mark.gpu
 def test_input_gradient_has_no_part_along_the_query():
