@@ -235,3 +235,34 @@ def test_router_scores_keep_the_tokens_for_q_proj_only(checkpoint, dtype):
         assert sizes == sorted(rest + ([120 * kept] if kept else [])), (frozen, sizes)
         dx, dk = torch.autograd.grad(s, (xin, k), ds)
         assert torch.equal(dx, full[0]) and torch.equal(dk, full[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+def test_balance_loss_of_a_module_captured_and_replayed(checkpoint):
+    """The module's balance loss with its gradients in a CUDA graph, replayed on other inputs and weights."""
+    m = make_mlp(torch.bfloat16, checkpoint)
+    x = randn(90, 256, seed=380, dtype=torch.bfloat16).requires_grad_()
+    valid = torch.ones(90, dtype=torch.bool, device="cuda")
+    leaves = [x, m.q_proj_16d.weight, m.block_keys_16d]
+
+    def step():
+        loss, counts = m.balance_loss(x, valid)
+        return [loss.detach(), counts, *torch.autograd.grad(loss, leaves, torch.full((), 0.5, device="cuda"))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x.copy_(randn(90, 256, seed=381, dtype=torch.bfloat16))
+        m.q_proj_16d.weight.mul_(1.5)
+        valid[40:60] = False
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in out]
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
