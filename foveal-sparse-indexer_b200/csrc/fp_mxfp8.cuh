@@ -6,9 +6,10 @@
 // rounding is the one to e4m3 (at most 2^-4 of the value, or 2^-10 of 2^k below the smallest normal), and a
 // copy does not depend on how the scale was computed.  Choosing the smallest k that fits 448 * 2^k never
 // clips the block's largest element (rounding its exponent down would clip mantissas above 1.75).  The upper
-// and lower clamp keep 2^k, 2^-k and every dequantised value (a multiple of 2^(k-9)) normal in fp32 and exact
-// in bf16.  The scale is stored as the byte k + 127.  Magnitudes of at least 248 * 2^120 would round to 2^128,
-// past fp32's range: they are held as 240 * 2^120, so that a finite value stays finite.
+// and lower clamp keep 2^k and 2^-k normal in fp32 and every dequantised value, a multiple of 2^(k-9), exact in
+// fp32 and bf16.  At k = -118 those are subnormal down to 2^-127: the kernels need a build that does not flush
+// subnormals to zero.  The scale is stored as the byte k + 127.  Magnitudes of at least 248 * 2^120 would round
+// to 2^128, past fp32's range: they are held as 240 * 2^120, so that a finite value stays finite.
 #pragma once
 #include "fp_internal.cuh"
 

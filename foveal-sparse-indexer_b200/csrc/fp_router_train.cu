@@ -92,7 +92,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // stays for many tiles of 32 tokens, with the block keys in shared memory once (loaded per 16 tokens they took
 // as long as the projection), a key serves four tokens from registers, and the normalisation factor and
 // (kKeep) the MXFP8 copy of x leave in the same pass over x.  Warp: one quarter of D, 16 tokens; then 4
-// tokens' scores.  HBM bound by x (16384 x 4096: 36 us, 4.1 TB/s; with the copy 55 us, 4.0 TB/s).
+// tokens' scores.  Bound by latency (16384 x 4096: 37 us, 3.6 TB/s at 29 % issue; 16384 x 8192 with the copy: 102 us,
+// 3.9 TB/s at 53 %): 128 registers leave 16 warps to an SM.
 // With the copy, x comes by TMA (64 columns x 16 tokens) into a ring that a warp keeps for itself and that runs
 // on through the scores of a tile (55 us; loads into registers 59 us: the quantisation leaves too few in
 // flight).  Without it, plain loads of two steps at a time do better (36 us; the ring 42 us: W_q's fragments
@@ -325,7 +326,8 @@ router_fwd_kernel(const __grid_constant__ CUtensorMap map, const __nv_bfloat16* 
 // order of sums (lane: columns 8 lane + 256 i, then a butterfly), so the same bits.  What held that kernel at
 // 270 us (16384 x 4096 fp32) were W_q's loads, 16 rows of them one after the other for each step of x; here a
 // step's W_q (256 columns) is in shared memory, copied one step ahead for the CTA's 32 tokens, and x is loaded
-// one step ahead.  Bound by the FMA units and shared memory (512 and 136 wavefronts a step) for fp32.
+// one step ahead.  134 us then, of which the FMA units take 29 and shared memory 29: 206 registers leave one CTA
+// of 8 warps to an SM (12.5 % of the warps, 47 % issue), too few to cover each other's latency.
 constexpr int kAnyTokens = 4;  // of a warp
 
 template <typename T>
@@ -540,7 +542,7 @@ __device__ __forceinline__ float4 ds4(const float* __restrict__ ds, int64_t t, i
 
 constexpr int kDqWarps = 8;
 constexpr int kDqTokens = 8 * kDqWarps;  // tokens of a CTA's tile
-constexpr int kDqMaxCtas = 296;
+constexpr int kDqMaxCtas = 296;  // two to each of the 148 SMs; also the partial sums of dK
 constexpr int kDqPieces = 3;                  // bf16 pieces of a packed dq
 constexpr int kDqTileBytes = kDqPieces * 512;  // 16 tokens of them
 
@@ -718,7 +720,9 @@ router_dq_kernel(const float* __restrict__ ds, const T* __restrict__ k16, const 
 // pieces of x (tokens 2t, 2t+1, 2t+8, 2t+9, columns 8g..) become the dWq product's A operand by permuting
 // halfwords of two tokens' words, without shared memory; dWq^T[d, j] stays in 32 registers over all tokens.
 // dx[tok, d] = dq Wq takes dq's fragments transposed (movmatrix) and Wq's from registers, its columns permuted
-// so that a lane stores 16 contiguous bytes.  wd warps (1, 2, 4) lie along the columns, 8 / wd along tokens;
+// so that a lane stores 16 contiguous bytes.  Neither HBM (16384 x 4096: 57 us, 3.9 TB/s; from the copy 16384 x 8192:
+// 127 us, 2.8 TB/s), issue (44 and 55 %) nor the tensor cores (48 and 41 %) is full: 16 warps to an SM wait for
+// one another's chains; W_q's fragments in shared memory, 3 or 4 stages made no difference.  wd warps (1, 2, 4) lie along the columns, 8 / wd along tokens;
 // the token groups' dWq are joined in shared memory, in order.
 constexpr int kXWarps = 8;
 
@@ -938,8 +942,8 @@ router_x_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* __restri
 // Pass 2, fp32, on the FMA units (32 per element): a thread owns 4 columns (their Wq and dWq in registers), dq (and
 // the copy's scales) of 32 tokens at a time in shared memory; tx threads (32, 64, 128) lie along the columns,
 // 128 / tx along tokens.  x runs through a ring of kFAhead tokens that a thread keeps for itself (cp.async).
-// Issue bound: 16384 x 4096 took 238 us with two loads in flight from registers, 166 us with the ring (3.2
-// TB/s); paired FMAs (fma.rn.f32x2) need fewer instructions, spill, and took 175 to 194 us.
+// 16384 x 4096 took 238 us with two loads in flight from registers, 160 us with the ring (3.1 TB/s; 67 % issue at 18 %
+// of the warps, of the time 58 us are FMAs: 168 registers leave three CTAs of 4 warps); paired FMAs (fma.rn.f32x2) need fewer instructions, spill, and took 175 to 194 us.
 constexpr int kFThreads = 128;
 constexpr int kFTokens = 32;
 constexpr int kFAhead = 8;

@@ -347,7 +347,7 @@ def balance_loss_fwd(scores: Optional[torch.Tensor], remote_indices: Optional[to
     lib = _lib.load()
     loss = state = None
     counts = torch.empty(num_blocks, dtype=torch.int64, device=dev)
-    # the state and the workspace are one buffer: at most 270 KB, kept until the backward pass
+    # the state and the workspace are one allocation of at most 270 KB, which lives until the backward pass
     at = (num_blocks * 4 + 4 + 15) // 16 * 16
     nbytes = lib.fp_balance_workspace_size(M, num_blocks)
     buf = torch.empty(at + nbytes, dtype=torch.uint8, device=dev)

@@ -116,8 +116,10 @@ def check_router(x: Tensor, q_proj: Tensor, block_keys: Tensor) -> None:
 
 def router_scores(x: Tensor, q_proj: Tensor, block_keys: Tensor, *, checkpoint: Optional[str] = None) -> Tensor:
     """``rms_norm(x q_proj^T) block_keys^T / 4`` per token, differentiable in all three: x [..., D] fp32 or
-    bf16, q_proj [16, D], block_keys [NB, 16] -> fp32 [..., NB].  With ``checkpoint="mxfp8"`` the backward
-    pass reads an 8-bit copy of x (it enters q_proj's gradient only)."""
+    bf16, q_proj [16, D], block_keys [NB, 16] -> fp32 [..., NB].  q_proj and block_keys are read in x's type (as
+    ``compute_router_scores`` does: fp32 weights next to bf16 x are rounded to bf16), their gradients leave in
+    their own.  With ``checkpoint="mxfp8"`` the backward pass reads an 8-bit copy of x (it enters q_proj's
+    gradient only; where q_proj takes none, neither x nor a copy is kept)."""
     check_checkpoint(checkpoint)
     check_router(x, q_proj, block_keys)
     # only q_proj's gradient reads the tokens: without it neither x nor a copy is kept
@@ -223,7 +225,8 @@ def balance_loss(scores: Tensor, remote_indices: Optional[Tensor], remote_counts
     remote_counts [...] the routes chosen from them (``select_blocks``).  With p_t the softmax of
     scores_t / temperature over the R = NB - base_blocks remote blocks, f_b block b's share of the slots and n
     the number of rows, ``loss = R sum_b f_b (1/n) sum_t p_tb``: 1 for an even load, R when one block takes
-    everything.  Temperatures from 1e-30 to 1e30, at most 2^20 slots to a list.  The gradient reaches the scores through p only.
+    everything.  Temperatures from 1e-30 to 1e30, at most 2^20 slots to a list.  The gradient reaches the scores
+    through p only.
 
     Rows whose ``valid`` is False or whose remote scores are all -inf are not counted in n and receive zeros;
     the slots are those of :func:`block_counts`, which leaves out the rows whose ``valid`` is False only.
