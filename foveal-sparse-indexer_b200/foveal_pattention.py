@@ -145,7 +145,7 @@ class _KeptBalance(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, module, x, wq, k16, valid):
-        base, T = module.base_blocks, module.temperature
+        base, T = int(module.base_blocks), float(module.temperature)
         scores, saved, _ = kernels.router_scores_train(x, wq, k16)
         loss, counts, state = checked_balance(scores, *module._token_routes(scores), base, T, valid)
         _, need_x, need_w, need_k, _ = ctx.needs_input_grad

@@ -266,3 +266,20 @@ def test_balance_loss_of_a_module_captured_and_replayed(checkpoint):
     torch.cuda.synchronize()
     got = [t.clone() for t in out]
     assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "mxfp8"])
+def test_balance_loss_of_a_module_with_a_temperature_of_another_type(checkpoint):
+    """A temperature that is a tensor or a numpy number counts as its value; one token alone has its gradients."""
+    import numpy as np
+
+    m = make_mlp(torch.float32, checkpoint)
+    x = randn(256, seed=390).requires_grad_()
+    out = []
+    for T in (0.5, torch.tensor(0.5), np.float32(0.5)):
+        m.temperature = T
+        loss, counts = m.balance_loss(x)
+        out.append([loss.detach(), counts, *torch.autograd.grad(loss, [x, m.q_proj_16d.weight, m.block_keys_16d])])
+    assert out[0][2].shape == (256,) and bool(out[0][2].any())
+    assert all(torch.equal(a, b) for o in out[1:] for a, b in zip(o, out[0]))
